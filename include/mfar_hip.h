@@ -494,6 +494,74 @@ int mfar_pipeline_result_view(mfar_pipeline* p, int64_t ticket, const int64_t** 
 /* the batch's stage-1 lists [Q, n_fields, k1] copied out like mfar_pipeline_result does for the final lists */
 int mfar_pipeline_lists(mfar_pipeline* p, int64_t ticket, int64_t* field_ids, float* field_scores, int on_device, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------------
+ * Operators of the encoder and of its training.  Handle-less; all pointers are DEVICE pointers on `device` unless said otherwise, the work is
+ * enqueued on `stream` without host synchronisation and may be captured into a graph; the caller owns every buffer, workspaces included (a
+ * workspace is in use until the work enqueued by the call has run: calls that may overlap need one each).  Arguments are checked before
+ * anything is enqueued.  The calling thread's current device is left as it was.
+ * ---------------------------------------------------------------------------------------------------------------------- */
+#define MFAR_DTYPE_F16 2   /* (of these operators only: an index holds F32 or BF16 rows) */
+
+/*
+ * Attention with a learned relative position bias by buckets (the gtr-t5 encoder's attention, modeling/util.py:22-36):
+ *   S[q][k] = scale <q, k> + table[bucket(k - pos(q))][h] over the visible keys, out = softmax(S) v;  pos(q) = q_start + q.
+ * A key is visible if key_mask (1 byte per key, 0 = hidden) leaves it and, when causal, k <= pos(q).  A row without visible keys gives zeros
+ * (and zero gradients); hidden keys may hold anything.
+ * Buckets: `each` = half of a side's buckets hold one distance each, distance d >= each falls into each + (number of borders <= d).  Causal: one
+ * side (distances behind the query); otherwise the upper half of the buckets is for keys behind the query's position.
+ */
+typedef struct mfar_attention {
+    int32_t dtype;                          /* MFAR_DTYPE_F32 / BF16 / F16: q, k, v, out and their gradients */
+    int32_t B, Lq, Lk, H, D;                /* D: multiple of 8, <= 128; B, H <= 65535 */
+    int32_t causal, n_buckets, n_borders;   /* n_buckets <= 256 (even unless causal) */
+    float scale;
+    const int32_t* borders;                 /* HOST [n_borders], ascending: n_borders = side - side / 2 - 1; last (or each) <= 1023 */
+    const float* table;                     /* [n_buckets, H] fp32 */
+    const void *q, *k, *v;                  /* element (b, l, h, d) at b * x_b + l * x_l + h * x_h + d; base and strides multiples of 16 bytes */
+    int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;
+    const uint8_t* key_mask;                /* [B, Lk] rows mask_b apart, or NULL: all visible */
+    int64_t mask_b;
+    const int32_t* q_start_each;            /* [B], or NULL: q_start for every sequence */
+    int32_t q_start;
+    void* out;                              /* [B, Lq, H, D] contiguous, 16-byte aligned */
+    void* out_lo;                           /* [B, Lq, H, D] or NULL: what out's rounding dropped (kept for the backward pass; unused for F32) */
+    float* lse;                             /* [B, H, Lq] or NULL: log2-sums for the backward pass */
+    void* workspace;                        /* mfar_attention_workspace_bytes(a, 0) bytes (may be NULL when that is 0) */
+    int64_t workspace_bytes;
+    /* backward only: out, out_lo, lse as the forward call left them */
+    const void* dout;
+    int64_t do_b, do_l, do_h;
+    void *dq, *dk, *dv;                     /* [B, Lq, H, D], [B, Lk, H, D] x 2, contiguous */
+    float* dtable;                          /* [n_buckets, H] or NULL: not wanted */
+} mfar_attention;
+int64_t mfar_attention_workspace_bytes(const mfar_attention* a, int backward);   /* < 0: MFAR_ERR_* */
+int mfar_attention_forward(int device, const mfar_attention* a, void* stream);
+int mfar_attention_backward(int device, const mfar_attention* a, void* stream);  /* bit-reproducible: no float atomics */
+
+/*
+ * 8-bit products with a scale for each token (row of x) and each output channel.
+ *   mfar_quantize_rows: scale[m] = max|x[m]| / 127, q[m] = rint(x[m] / scale[m]), ties to even; rows of q ldq bytes apart.  A row of zeros gets
+ *   scale 0, a row with an infinity or NaN scale NaN and zeros.
+ *   mfar_int8_linear: y = quantize_rows(x) wq' scaled by both scales (+ bias), rounded once to x's type.
+ * x [M, K] rows ldx elements apart; wq [N, K] contiguous; w_scale [N]; bias [N] fp32 or NULL; y [M, N] contiguous, of x's type.  K <= 131072.
+ */
+int mfar_quantize_rows(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int8_t* q, int64_t ldq, float* scale, void* stream);
+int64_t mfar_int8_linear_workspace_bytes(int64_t M, int K);
+int mfar_int8_linear(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int N, const int8_t* wq, const float* w_scale,
+                     const float* bias, void* y, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Distillation from a teacher's top scores: p = softmax(scores / tau) over a row's ids >= 0, q = softmax(student / tau) over its N columns;
+ * loss[t] = tau^2 KL(p || q).  A row without ids: loss and gradient 0.  An id >= N: the row's loss and gradient are NaN.  An id may repeat.
+ * student [T, N] rows ld elements apart; ids [T, K] int64, scores [T, K] fp32, K <= 1024; prob [T, K] and lse [T] are kept for the backward
+ * pass; dstudent [T, N] contiguous, of the student's type; dloss [T].
+ */
+int64_t mfar_distill_workspace_bytes(int64_t T, int64_t N);
+int mfar_distill_forward(int device, const void* student, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, const float* scores, int K,
+                         float tau, float* loss, float* prob, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int mfar_distill_backward(int device, const void* student, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, int K, float tau,
+                          const float* prob, const float* lse, const float* dloss, void* dstudent, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

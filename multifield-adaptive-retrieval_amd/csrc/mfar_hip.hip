@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "mfar_hip.h"
+#include "mfar_error.h"
 #include "mfar_policy.h"
 #include "mfar_select.h"
 #include "mfar_screen.h"
@@ -26,6 +27,13 @@ static thread_local std::string g_err;
 static int fail(int code, const std::string& msg) {
     g_err = msg;
     return code;
+}
+int mfar_report(int code, const char* msg) {
+    try {
+        return fail(code, msg);
+    } catch (...) {      // no memory left for the text: the code alone
+        return code;
+    }
 }
 #define HIPCHK(expr)                                                                                  \
     do {                                                                                              \

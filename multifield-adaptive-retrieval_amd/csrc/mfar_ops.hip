@@ -1,0 +1,275 @@
+// mfar_ops.hip -- host side of the encoder / training operators of libmfar_hip.so (include/mfar_hip.h, last section).
+// gfx950 only.  Every entry point returns an error code; nothing throws across the ABI.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdio>
+
+#include "mfar_hip.h"
+#include "mfar_error.h"
+#include "mfar_attention.h"
+#include "mfar_distill.h"
+#include "mfar_int8.h"
+
+namespace {
+
+int bad(const char* msg) { return mfar_report(MFAR_ERR_INVALID, msg); }
+int hip_failed(const char* what, hipError_t e) {
+    (void)hipGetLastError();     // reported here: not left behind for the next call
+    char msg[256];
+    std::snprintf(msg, sizeof msg, "%s: %s", what, hipGetErrorString(e));
+    return mfar_report(MFAR_ERR_HIP, msg);
+}
+
+// makes `device` current for a scope
+struct OnDevice {
+    int before = -1;
+    hipError_t err;
+    explicit OnDevice(int device) {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device);
+        else if (err == hipSuccess) before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+#define ON_DEVICE(device)                                                              \
+    OnDevice on_device_(device);                                                       \
+    if (on_device_.err != hipSuccess) return hip_failed("hipSetDevice", on_device_.err)
+#define LAUNCHED(what)                                                \
+    do {                                                              \
+        const hipError_t e_ = hipGetLastError();                      \
+        if (e_ != hipSuccess) return hip_failed(what, e_);            \
+    } while (0)
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int type_size(int dtype) { return dtype == MFAR_DTYPE_F32 ? 4 : (dtype == MFAR_DTYPE_BF16 || dtype == MFAR_DTYPE_F16) ? 2 : 0; }
+
+// a kernel that may need more than the default 64 KB of dynamic LDS: allowed once per device and kernel
+template <typename F> hipError_t allow_lds(F kernel, std::atomic<uint32_t>& done) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint32_t bit = dev < 32 ? 1u << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return hipSuccess;
+    e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 156 * 1024);   // (some have a few static bytes)
+    if (e == hipSuccess && bit) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+// (kernels that share a type have a flag each: the address of one instance is a template argument)
+template <auto KERNEL, typename P> int launch(const char* name, dim3 grid, size_t lds, hipStream_t st, const P& p) {
+    if (lds > 64 * 1024) {
+        static std::atomic<uint32_t> done{0};
+        const hipError_t e = allow_lds(KERNEL, done);
+        if (e != hipSuccess) return hip_failed(name, e);
+    }
+    KERNEL<<<grid, dim3(256), lds, st>>>(p);
+    LAUNCHED(name);
+    return MFAR_OK;
+}
+
+// ---- attention --------------------------------------------------------------------------------------------------------------------------
+int check_attention(const mfar_attention* a, bool backward) {
+    if (!a) return bad("NULL arguments");
+    const int es = type_size(a->dtype);
+    if (!es) return bad("dtype must be F32, BF16 or F16");
+    if (a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 1 || a->B > 65535 || a->H > 65535) return bad("B, Lq, Lk must be >= 0, H >= 1, B and H <= 65535");
+    if (a->D < 8 || a->D > 128 || a->D % 8) return bad("D must be a multiple of 8, at most 128");
+    if (a->Lq > (1 << 30) || a->Lk > (1 << 30)) return bad("at most 2^30 queries and keys");
+    if (a->q_start < -(1 << 30) || a->q_start > (1 << 30)) return bad("q_start out of range");
+    if (a->n_buckets < 2 || a->n_buckets > 256 || (!a->causal && (a->n_buckets % 2 || a->n_buckets < 4))) return bad("n_buckets must be 2..256, even and >= 4 unless causal");
+    const int side = a->causal ? a->n_buckets : a->n_buckets / 2, each = side / 2;
+    if (a->n_borders != side - each - 1 || (a->n_borders && !a->borders)) return bad("n_borders must be side - side / 2 - 1");
+    for (int j = 0; j < a->n_borders; ++j)
+        if (a->borders[j] < each || (j && a->borders[j] < a->borders[j - 1])) return bad("borders must ascend from the first shared distance");
+    if ((a->n_borders ? a->borders[a->n_borders - 1] : each) > 1023) return bad("the last bucket must begin at a distance <= 1023");
+    if (a->B == 0 || a->Lq == 0) return MFAR_OK;
+    if (!a->q || !a->out || !a->table || (a->Lk && (!a->k || !a->v))) return bad("NULL tensor");
+    const int64_t strides[] = {a->q_b, a->q_l, a->q_h, a->k_b, a->k_l, a->k_h, a->v_b, a->v_l, a->v_h};
+    for (int64_t s : strides)
+        if (s * es % 16) return bad("strides must be multiples of 16 bytes");
+    if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) || !aligned16(a->out_lo)) return bad("tensors must be 16-byte aligned");
+    if (backward) {
+        if (!a->dout || !a->dq || !a->lse || (a->Lk && (!a->dk || !a->dv))) return bad("NULL gradient or lse");
+        if (a->do_b * es % 16 || a->do_l * es % 16 || a->do_h * es % 16) return bad("strides must be multiples of 16 bytes");
+        if (!aligned16(a->dout) || !aligned16(a->dq) || !aligned16(a->dk) || !aligned16(a->dv)) return bad("tensors must be 16-byte aligned");
+    }
+    return MFAR_OK;
+}
+AttnParams attention_params(const mfar_attention* a) {
+    AttnParams p = {};
+    p.q = a->q, p.k = a->k, p.v = a->v, p.o = a->out, p.dout = a->dout;
+    p.out = a->out, p.dq = a->dq, p.dk = a->dk, p.dv = a->dv;
+    p.o_lo = p.out_lo = a->dtype == MFAR_DTYPE_F32 ? nullptr : a->out_lo;
+    p.q_b = a->q_b, p.q_l = a->q_l, p.q_h = a->q_h, p.k_b = a->k_b, p.k_l = a->k_l, p.k_h = a->k_h, p.v_b = a->v_b, p.v_l = a->v_l, p.v_h = a->v_h;
+    p.do_b = a->do_b, p.do_l = a->do_l, p.do_h = a->do_h;
+    p.table = a->table, p.mask = a->key_mask, p.mask_b = a->mask_b, p.start_ptr = a->q_start_each, p.start = a->q_start, p.lse = a->lse;
+    p.B = a->B, p.Lq = a->Lq, p.Lk = a->Lk, p.H = a->H, p.D = a->D, p.causal = a->causal != 0, p.scale = a->scale;
+    p.n_buckets = a->n_buckets, p.n_side = a->causal ? a->n_buckets : a->n_buckets / 2, p.each = p.n_side / 2, p.n_borders = a->n_borders;
+    for (int j = 0; j < a->n_borders; ++j) p.borders[j] = a->borders[j];
+    p.sat = a->n_borders ? a->borders[a->n_borders - 1] : p.each;
+    return p;
+}
+int64_t drow_bytes(const mfar_attention* a) { return ((int64_t)a->B * a->H * a->Lq * 4 + 15) / 16 * 16; }
+size_t lut_bytes(const AttnParams& p) { return (size_t)(2 * p.sat + 1) * 4; }
+
+template <typename T, int DP> int attention_forward(const AttnParams& p, hipStream_t st) {
+    const size_t lds = 2ull * AT_TILE * DP * sizeof(T) + 64 * 8 + lut_bytes(p);
+    const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
+    if constexpr (sizeof(T) == 2)
+        if (p.out_lo) return launch<mfar_attn_forward_kernel<T, DP, true>>("mfar_attn_forward_kernel", grid, lds, st, p);
+    return launch<mfar_attn_forward_kernel<T, DP, false>>("mfar_attn_forward_kernel", grid, lds, st, p);
+}
+template <typename T, int DP> int attention_backward(const AttnParams& p, float* dtable, hipStream_t st) {
+    const size_t tiles = 2ull * AT_TILE * DP * sizeof(T);
+    const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
+    int rc = launch<mfar_attn_dq_kernel<T, DP>>("mfar_attn_dq_kernel", grid, tiles + 64 * 8 + lut_bytes(p) * (p.dpart ? 9 : 1), st, p);
+    if (rc != MFAR_OK) return rc;
+    if (p.Lk) {
+        rc = launch<mfar_attn_dkv_kernel<T, DP>>("mfar_attn_dkv_kernel", dim3(cdiv(p.Lk, AT_COLS), p.H, p.B), tiles + 2 * AT_TILE * 4 + lut_bytes(p), st, p);
+        if (rc != MFAR_OK) return rc;
+    }
+    if (p.dpart) {
+        mfar_attn_dtable_kernel<<<p.H * p.n_buckets, AT_BLOCK, 0, st>>>(p.dpart, (int)(grid.x * grid.z), p.H, p.n_buckets, dtable);
+        LAUNCHED("mfar_attn_dtable_kernel");
+    }
+    return MFAR_OK;
+}
+#define FOR_TYPE_AND_DIM(FN, ...)                                                                                                     \
+    (a->dtype == MFAR_DTYPE_F32    ? (a->D <= 32 ? FN<float, 32>(__VA_ARGS__) : a->D <= 64 ? FN<float, 64>(__VA_ARGS__) : FN<float, 128>(__VA_ARGS__)) \
+     : a->dtype == MFAR_DTYPE_BF16 ? (a->D <= 32 ? FN<__bf16, 32>(__VA_ARGS__) : a->D <= 64 ? FN<__bf16, 64>(__VA_ARGS__) : FN<__bf16, 128>(__VA_ARGS__)) \
+                                   : (a->D <= 32 ? FN<_Float16, 32>(__VA_ARGS__) : a->D <= 64 ? FN<_Float16, 64>(__VA_ARGS__) : FN<_Float16, 128>(__VA_ARGS__)))
+#define FOR_TYPE(dtype, FN, ...) ((dtype) == MFAR_DTYPE_F32 ? FN<float>(__VA_ARGS__) : (dtype) == MFAR_DTYPE_BF16 ? FN<__bf16>(__VA_ARGS__) : FN<_Float16>(__VA_ARGS__))
+
+// ---- distillation -----------------------------------------------------------------------------------------------------------------------
+// A row is cut into pieces of at least 4096 columns while there are fewer than 2048 blocks (8 per CU).
+int distill_chunk(int64_t T, int64_t N) {
+    const int64_t splits = std::max<int64_t>(1, std::min(cdiv(2048, std::max<int64_t>(1, T)), cdiv(N, 4096)));
+    return (int)(cdiv(cdiv(N, splits), 64) * 64);
+}
+template <typename T> int distill_forward(const DistillParams& p, hipStream_t st) {
+    int rc = launch<mfar_distill_forward_kernel<T>>("mfar_distill_forward_kernel", dim3(p.T, p.splits), 0, st, p);
+    if (rc == MFAR_OK && p.splits > 1) rc = launch<mfar_distill_join_kernel<T>>("mfar_distill_join_kernel", dim3(p.T), 0, st, p);
+    return rc;
+}
+template <typename T> int distill_backward(const DistillParams& p, hipStream_t st) {
+    return launch<mfar_distill_backward_kernel<T>>("mfar_distill_backward_kernel", dim3(p.T, p.splits), 0, st, p);
+}
+int check_distill(const void* x, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, int K, float tau) {
+    if (!type_size(dtype)) return bad("dtype must be F32, BF16 or F16");
+    if (T < 0 || T > 0x7fffffff || N < 1 || N > (1 << 30)) return bad("T must be 0..2^31 - 1, N 1..2^30");
+    if (K < 1 || K > DI_MAX_K) return bad("K must be 1..1024");
+    if (!(tau > 0.0f) || tau > 3.0e38f) return bad("the temperature must be positive and finite");
+    if (T && (!x || !ids)) return bad("NULL tensor");
+    if (T > 1 && ld < 0) return bad("rows must not run backwards");
+    return MFAR_OK;
+}
+
+// ---- 8-bit linear -----------------------------------------------------------------------------------------------------------------------
+template <typename T> int quantize_rows(const void* x, int64_t ldx, int64_t M, int K, int8_t* q, int64_t ldq, float* scale, int pad, hipStream_t st) {
+    mfar_quantize_rows_kernel<T><<<cdiv(M, 4), 256, 0, st>>>((const T*)x, ldx, (int)M, K, (signed char*)q, ldq, scale, pad);
+    LAUNCHED("mfar_quantize_rows_kernel");
+    return MFAR_OK;
+}
+template <typename T> int int8_gemm(const Int8Params& p, hipStream_t st) {
+    return launch<mfar_int8_gemm_kernel<T>>("mfar_int8_gemm_kernel", dim3(cdiv(p.N, Q8_TILE), cdiv(p.M, Q8_TILE)), 0, st, p);
+}
+int check_rows(const void* x, int dtype, int64_t ldx, int64_t M, int K) {
+    if (!type_size(dtype)) return bad("dtype must be F32, BF16 or F16");
+    if (M < 0 || M > (1 << 23) || K < 1 || K > Q8_MAX_K) return bad("M must be 0..2^23, K 1..131072");
+    if (M && !x) return bad("NULL tensor");
+    if (M > 1 && ldx < 0) return bad("rows must not run backwards");
+    return MFAR_OK;
+}
+int64_t padded_k(int K) { return cdiv(K, 128) * 128; }
+
+}  // namespace
+
+extern "C" int64_t mfar_attention_workspace_bytes(const mfar_attention* a, int backward) {
+    const int rc = check_attention(a, false);
+    if (rc != MFAR_OK) return rc;
+    if (!backward || a->B == 0 || a->Lq == 0) return 0;
+    return drow_bytes(a) + (a->dtable ? cdiv(a->Lq, AT_COLS) * a->B * a->H * a->n_buckets * 4 : 0);
+}
+extern "C" int mfar_attention_forward(int device, const mfar_attention* a, void* stream) {
+    int rc = check_attention(a, false);
+    if (rc != MFAR_OK || a->B == 0 || a->Lq == 0) return rc;
+    ON_DEVICE(device);
+    const AttnParams p = attention_params(a);
+    return FOR_TYPE_AND_DIM(attention_forward, p, (hipStream_t)stream);
+}
+extern "C" int mfar_attention_backward(int device, const mfar_attention* a, void* stream) {
+    int rc = check_attention(a, true);
+    if (rc != MFAR_OK) return rc;
+    if (a->B == 0 || a->Lq == 0) return bad("an empty batch has no backward pass");
+    if (!a->workspace || a->workspace_bytes < mfar_attention_workspace_bytes(a, 1)) return bad("workspace too small");
+    ON_DEVICE(device);
+    AttnParams p = attention_params(a);
+    p.drow = (float*)a->workspace;
+    p.dpart = a->dtable ? (float*)((char*)a->workspace + drow_bytes(a)) : nullptr;
+    return FOR_TYPE_AND_DIM(attention_backward, p, a->dtable, (hipStream_t)stream);
+}
+
+extern "C" int mfar_quantize_rows(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int8_t* q, int64_t ldq, float* scale, void* stream) {
+    const int rc = check_rows(x, dtype, ldx, M, K);
+    if (rc != MFAR_OK || M == 0) return rc;
+    if (!q || !scale) return bad("NULL output");
+    if (ldq < K) return bad("ldq must be at least K");
+    ON_DEVICE(device);
+    return FOR_TYPE(dtype, quantize_rows, x, ldx, M, K, q, ldq, scale, 0, (hipStream_t)stream);
+}
+extern "C" int64_t mfar_int8_linear_workspace_bytes(int64_t M, int K) {
+    if (M < 0 || K < 1) return bad("M must be >= 0, K >= 1");
+    return M * padded_k(K) + cdiv(M * 4, 16) * 16;
+}
+extern "C" int mfar_int8_linear(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int N, const int8_t* wq, const float* w_scale,
+                                const float* bias, void* y, void* workspace, int64_t workspace_bytes, void* stream) {
+    int rc = check_rows(x, dtype, ldx, M, K);
+    if (rc != MFAR_OK) return rc;
+    if (N < 0 || N > (1 << 23)) return bad("N must be 0..2^23");
+    if (M == 0 || N == 0) return MFAR_OK;
+    if (!wq || !w_scale || !y) return bad("NULL tensor");
+    if (!workspace || !aligned16(workspace) || workspace_bytes < mfar_int8_linear_workspace_bytes(M, K)) return bad("workspace too small or not 16-byte aligned");
+    ON_DEVICE(device);
+    const int64_t Kp = padded_k(K);
+    int8_t* xq = (int8_t*)workspace;
+    float* xs = (float*)((char*)workspace + M * Kp);
+    hipStream_t st = (hipStream_t)stream;
+    rc = FOR_TYPE(dtype, quantize_rows, x, ldx, M, K, xq, Kp, xs, 1, st);
+    if (rc != MFAR_OK) return rc;
+    const Int8Params p = {(const signed char*)xq, (const signed char*)wq, xs, w_scale, bias, y, (long long)Kp, (long long)K, (int)M, N, K, (int)Kp};
+    return FOR_TYPE(dtype, int8_gemm, p, st);
+}
+
+extern "C" int64_t mfar_distill_workspace_bytes(int64_t T, int64_t N) {
+    if (T < 0 || N < 1 || N > (1 << 30)) return bad("T must be >= 0, N 1..2^30");
+    const int64_t splits = cdiv(N, distill_chunk(T, N));
+    return splits > 1 ? T * splits * 8 : 0;
+}
+extern "C" int mfar_distill_forward(int device, const void* student, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, const float* scores,
+                                    int K, float tau, float* loss, float* prob, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    const int rc = check_distill(student, dtype, ld, T, N, ids, K, tau);
+    if (rc != MFAR_OK || T == 0) return rc;
+    if (!scores || !loss || !prob || !lse) return bad("NULL tensor");
+    const int64_t need = mfar_distill_workspace_bytes(T, N);
+    if (need && (!workspace || workspace_bytes < need)) return bad("workspace too small");
+    ON_DEVICE(device);
+    DistillParams p = {};
+    p.x = student, p.x_row = ld, p.ids = (const long long*)ids, p.scores = scores, p.loss = loss, p.prob = prob, p.lse = lse, p.part = (float*)workspace;
+    p.T = (int)T, p.N = (int)N, p.K = K, p.chunk = distill_chunk(T, N), p.splits = (int)cdiv(N, p.chunk), p.tau = tau;
+    return FOR_TYPE(dtype, distill_forward, p, (hipStream_t)stream);
+}
+extern "C" int mfar_distill_backward(int device, const void* student, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, int K, float tau,
+                                     const float* prob, const float* lse, const float* dloss, void* dstudent, void* stream) {
+    const int rc = check_distill(student, dtype, ld, T, N, ids, K, tau);
+    if (rc != MFAR_OK || T == 0) return rc;
+    if (!prob || !lse || !dloss || !dstudent) return bad("NULL tensor");
+    ON_DEVICE(device);
+    DistillParams p = {};
+    p.x = student, p.x_row = ld, p.ids = (const long long*)ids, p.g = dloss, p.prob = (float*)prob, p.lse = (float*)lse, p.dx = dstudent;
+    p.T = (int)T, p.N = (int)N, p.K = K, p.chunk = distill_chunk(T, N), p.splits = (int)cdiv(N, p.chunk), p.tau = tau;
+    return FOR_TYPE(dtype, distill_backward, p, (hipStream_t)stream);
+}

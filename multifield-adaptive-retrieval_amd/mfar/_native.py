@@ -19,7 +19,7 @@ CSRC = os.path.join(_PKG, "csrc")
 
 MFAR_OK = 0
 ERR_NAMES = {-1: "MFAR_ERR_INVALID", -2: "MFAR_ERR_HIP", -3: "MFAR_ERR_NOMEM", -4: "MFAR_ERR_UNSUPPORTED"}
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 MAX_K, MAX_FIELDS = 128, 32
 
 
@@ -41,6 +41,18 @@ _lib = None
 
 _c = ctypes
 _vp, _i, _i64, _f32p = _c.c_void_p, _c.c_int, _c.c_int64, _c.c_void_p
+
+
+
+class Attention(_c.Structure):
+    """mfar_attention of include/mfar_hip.h."""
+    _fields_ = ([(n, _c.c_int32) for n in ("dtype", "B", "Lq", "Lk", "H", "D", "causal", "n_buckets", "n_borders")] +
+                [("scale", _c.c_float), ("borders", _c.POINTER(_c.c_int32)), ("table", _vp), ("q", _vp), ("k", _vp), ("v", _vp)] +
+                [(n, _i64) for n in ("q_b", "q_l", "q_h", "k_b", "k_l", "k_h", "v_b", "v_l", "v_h")] +
+                [("key_mask", _vp), ("mask_b", _i64), ("q_start_each", _vp), ("q_start", _c.c_int32), ("out", _vp), ("out_lo", _vp), ("lse", _vp),
+                 ("workspace", _vp), ("workspace_bytes", _i64), ("dout", _vp), ("do_b", _i64), ("do_l", _i64), ("do_h", _i64),
+                 ("dq", _vp), ("dk", _vp), ("dv", _vp), ("dtable", _vp)])
+
 
 # name -> (restype, argtypes); must list every symbol declared in include/mfar_hip.h
 SIGNATURES = {
@@ -109,6 +121,15 @@ SIGNATURES = {
     "mfar_pipeline_flush": (_i, [_vp]),
     "mfar_pipeline_result": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _vp]),
     "mfar_pipeline_lists": (_i, [_vp, _i64, _vp, _vp, _i, _vp]),
+    "mfar_attention_workspace_bytes": (_i64, [_c.POINTER(Attention), _i]),
+    "mfar_attention_forward": (_i, [_i, _c.POINTER(Attention), _vp]),
+    "mfar_attention_backward": (_i, [_i, _c.POINTER(Attention), _vp]),
+    "mfar_quantize_rows": (_i, [_i, _vp, _i, _i64, _i64, _i, _vp, _i64, _vp, _vp]),
+    "mfar_int8_linear_workspace_bytes": (_i64, [_i64, _i]),
+    "mfar_int8_linear": (_i, [_i, _vp, _i, _i64, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mfar_distill_workspace_bytes": (_i64, [_i64, _i64]),
+    "mfar_distill_forward": (_i, [_i, _vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _c.c_float, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mfar_distill_backward": (_i, [_i, _vp, _i, _i64, _i64, _i64, _vp, _i, _c.c_float, _vp, _vp, _vp, _vp, _vp]),
     "mfar_pipeline_result_view": (_i, [_vp, _i64, _c.POINTER(_vp), _c.POINTER(_vp), _c.POINTER(_vp), _c.POINTER(_vp), _c.POINTER(_vp)]),
 }
 
@@ -146,6 +167,34 @@ def lib():
 def check(rc: int):
     if rc != MFAR_OK:
         raise MfarError(rc, lib().mfar_last_error().decode("utf-8", "replace"))
+
+
+def op_dtype(t) -> int:
+    """Type code of a tensor handed to an encoder / training operator."""
+    import torch
+    code = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}.get(t.dtype)
+    if code is None:
+        raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def op_device(*tensors) -> int:
+    """The one GPU all of an operator's tensors live on (None entries are skipped); there is no CPU form."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"expected a tensor on the GPU, got one on {t.device}")
+        if dev is not None and t.device.index != dev:
+            raise ValueError(f"tensors live on cuda:{dev} and {t.device}")
+        dev = t.device.index
+    return dev
+
+
+def op_stream(device: int) -> int:
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def device_count() -> int:

@@ -15,6 +15,8 @@ from typing import Optional
 
 import torch
 
+from mfar import _native
+
 
 def _all_gather_cat(t: torch.Tensor) -> torch.Tensor:
     import torch.distributed as dist
@@ -79,3 +81,72 @@ class HybridContrastiveLoss(torch.nn.Module):
             import torch.distributed.nn.functional as dist_f
             nll = dist_f.all_reduce(nll) / dist.get_world_size()
         return nll
+
+
+class _TopKDistillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, student, ids, scores, tau):
+        dev = student.device.index
+        T, N = student.shape
+        K = ids.shape[1]
+        x = student if student.stride(1) == 1 or N == 1 else student.contiguous()
+        loss, lse = (torch.empty(T, dtype=torch.float32, device=x.device) for _ in range(2))
+        prob = torch.empty(T, K, dtype=torch.float32, device=x.device)
+        L = _native.lib()
+        n = L.mfar_distill_workspace_bytes(T, N)
+        work = torch.empty(max(0, n), dtype=torch.uint8, device=x.device)
+        _native.check(L.mfar_distill_forward(dev, x.data_ptr(), _native.op_dtype(x), x.stride(0), T, N, ids.data_ptr(), scores.data_ptr(), K, tau,
+                                             loss.data_ptr(), prob.data_ptr(), lse.data_ptr(), work.data_ptr(), n, _native.op_stream(dev)))
+        ctx.save_for_backward(x, ids, prob, lse)
+        ctx.tau = tau
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, ids, prob, lse = ctx.saved_tensors
+        dev = x.device.index
+        T, N = x.shape
+        dx = torch.empty(T, N, dtype=x.dtype, device=x.device)
+        dloss = dloss.float().contiguous()
+        _native.check(_native.lib().mfar_distill_backward(dev, x.data_ptr(), _native.op_dtype(x), x.stride(0), T, N, ids.data_ptr(), ids.shape[1], ctx.tau,
+                                                          prob.data_ptr(), lse.data_ptr(), dloss.data_ptr(), dx.data_ptr(), _native.op_stream(dev)))
+        return dx, None, None, None
+
+
+def topk_distillation(student: torch.Tensor, teacher_ids: torch.Tensor, teacher_scores: torch.Tensor, *, temperature: float = 1.0) -> torch.Tensor:
+    """temperature^2 KL(teacher || student) of every row -> [T] fp32, differentiable in the student's scores (mfar_distill_* of
+    include/mfar_hip.h).  The teacher is known by its top list alone, as `MultiFieldIndex.search` returns it: its distribution is the softmax
+    over a row's listed scores / temperature; the student's is the softmax over all of the row's N columns.
+
+    student [T, N] float32 / float16 / bfloat16 on the GPU; teacher_ids [T, K] int64 or int32 columns, K <= 1024, negative: no entry (short
+    lists); teacher_scores [T, K], used in fp32, no gradient.  A row without entries has loss 0 and gradient 0; an id past the last column
+    makes its row NaN; a repeated id adds up."""
+    dev = _native.op_device(student, teacher_ids, teacher_scores)
+    if student.dim() != 2 or student.shape[1] < 1 or student.shape[1] > 2 ** 30:
+        raise ValueError(f"expected student scores [T, N], 1 <= N <= 2^30, got {tuple(student.shape)}")
+    if teacher_ids.dtype not in (torch.int64, torch.int32) or teacher_ids.dim() != 2 or teacher_ids.shape[0] != student.shape[0]:
+        raise ValueError(f"expected int64 or int32 teacher_ids [{student.shape[0]}, K], got {teacher_ids.dtype} {tuple(teacher_ids.shape)}")
+    if not 1 <= teacher_ids.shape[1] <= 1024:
+        raise ValueError(f"a teacher's list has 1 to 1024 entries, got {teacher_ids.shape[1]}")
+    if teacher_scores.shape != teacher_ids.shape or not teacher_scores.is_floating_point():
+        raise ValueError(f"expected float teacher_scores {tuple(teacher_ids.shape)}, got {teacher_scores.dtype} {tuple(teacher_scores.shape)}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"the temperature must be positive and finite, got {temperature}")
+    _native.op_dtype(student)
+    with torch.cuda.device(dev):
+        return _TopKDistillation.apply(student, teacher_ids.to(torch.int64).contiguous(), teacher_scores.detach().float().contiguous(), float(temperature))
+
+
+class TopKDistillationLoss(torch.nn.Module):
+    """`topk_distillation` over a batch of queries: reduction "mean" (over the rows), "sum" or "none"."""
+
+    def __init__(self, temperature: float = 1.0, reduction: str = "mean"):
+        super().__init__()
+        if reduction not in ("mean", "sum", "none"):
+            raise ValueError(f"reduction must be mean, sum or none, got {reduction}")
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, student_scores: torch.Tensor, teacher_ids: torch.Tensor, teacher_scores: torch.Tensor) -> torch.Tensor:
+        loss = topk_distillation(student_scores, teacher_ids, teacher_scores, temperature=self.temperature)
+        return loss if self.reduction == "none" else (loss.mean() if self.reduction == "mean" else loss.sum())

@@ -1,0 +1,67 @@
+"""8-bit linear layers for inference on the GPU (mfar_quantize_rows / mfar_int8_linear of include/mfar_hip.h).
+
+One scale per token, computed on the fly, one per output channel, laid out once; exact integer sums on the matrix units at twice the rate of
+16-bit types.  There is no CPU form and no gradient: the layers serve forwards under `torch.no_grad()`.
+"""
+from typing import Optional, Tuple
+
+import torch
+
+from mfar import _native
+
+MAX_K = 131072
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """[..., K] as a 2-D view of rows with contiguous elements."""
+    r = x.reshape(-1, x.shape[-1])
+    return r if r.stride(1) == 1 or r.size(1) == 1 else r.contiguous()
+
+
+def _check(x: torch.Tensor) -> None:
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_K:
+        raise ValueError(f"expected [..., K] with K in 1..{MAX_K}, got {tuple(x.shape)}")
+    _native.op_dtype(x)
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("the 8-bit layers have no gradient: call them under torch.no_grad()")
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [..., K] float32 / float16 / bfloat16 -> (q int8 [..., K], scale fp32 [...]): scale = max|row| / 127, q = rint(row / scale), ties to
+    even.  A row of zeros has scale 0; a row with an infinity or NaN has scale NaN and zeros."""
+    dev = _native.op_device(x)
+    _check(x)
+    K = x.shape[-1]
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    r = _rows(x)
+    _native.check(_native.lib().mfar_quantize_rows(dev, r.data_ptr(), _native.op_dtype(x), r.stride(0), r.shape[0], K, q.data_ptr(), K, scale.data_ptr(),
+                                                   _native.op_stream(dev)))
+    return q, scale
+
+
+def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [..., K] times 8-bit weights wq [N, K] with one scale per channel w_scale [N] (+ bias [N]) -> [..., N] of x's type, every token quantised
+    by its own scale on the way (`quantize_rows`); rounded once."""
+    dev = _native.op_device(x, wq, w_scale, bias)
+    _check(x)
+    K = x.shape[-1]
+    if wq.dtype != torch.int8 or wq.dim() != 2 or wq.shape[1] != K:
+        raise ValueError(f"expected int8 weights [N, {K}], got {wq.dtype} {tuple(wq.shape)}")
+    N = wq.shape[0]
+    if w_scale.dtype != torch.float32 or w_scale.shape != (N,):
+        raise ValueError(f"expected float32 scales [{N}], got {w_scale.dtype} {tuple(w_scale.shape)}")
+    if bias is not None:
+        if not bias.is_floating_point() or bias.shape != (N,):
+            raise ValueError(f"expected a float bias [{N}], got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.detach().float().contiguous()
+    wq, w_scale = wq.contiguous(), w_scale.contiguous()
+    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    r = _rows(x)
+    L = _native.lib()
+    n = L.mfar_int8_linear_workspace_bytes(r.shape[0], K)
+    with torch.cuda.device(dev):
+        work = torch.empty(n, dtype=torch.uint8, device=x.device)
+        _native.check(L.mfar_int8_linear(dev, r.data_ptr(), _native.op_dtype(x), r.stride(0), r.shape[0], K, N, wq.data_ptr(), w_scale.data_ptr(),
+                                         bias.data_ptr() if bias is not None else None, y.data_ptr(), work.data_ptr(), n, _native.op_stream(dev)))
+    return y
