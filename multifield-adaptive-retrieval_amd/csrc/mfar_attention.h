@@ -21,6 +21,14 @@
 #define AT_COLS 128
 #define AT_TILE 64        // keys (queries) staged in LDS per step
 #define AT_MAX_BORDERS 128
+#define AT_MAX_STRIDE (1 << 22)
+// The running maximum of the softmax follows a tile's only when that is 2^8 over it: probabilities stay under 256 (fp16 holds them as exactly as
+// those under 1), and the accumulated output is hardly ever rescaled.
+#define AT_SLACK 8.0f
+
+// Waves per SIMD the register budget is set for.  From 2 on (256 registers) the compiler keeps accumulators where the vector unit reaches them;
+// with the whole file for one wave it parks them in accumulation registers and copies every score back and forth.
+constexpr int at_waves(int size, int dp, int want) { return size == 2 && dp <= 64 ? want : (size == 2 ? 2 : (dp <= 64 ? 2 : 1)); }
 
 struct AttnParams {
     const void *q, *k, *v, *o, *o_lo, *dout;
@@ -59,19 +67,45 @@ template <int DP> __device__ __forceinline__ int at_swz(int r) {
 }
 template <typename T, int DP> __device__ __forceinline__ T* at_at(T* tile, int r, int c) { return tile + r * DP + ((c ^ at_swz<DP>(r)) << 3); }
 
-// rows [r0, r0 + AT_TILE) of one (batch, head) -> LDS; rows whose bit of `bits` is 0 and dims >= D become zeros (a masked row may hold
-// anything, also NaN: it must not reach a product)
-template <typename T, int DP>
-__device__ __forceinline__ void at_stage(T* tile, const T* src, long long stride, int r0, u64 bits, int D) {
-    constexpr int CH = DP / 8;
+// Tiles of AT_TILE rows of one (batch, head) on their way to LDS: fetch() loads one into registers (ahead of the step that needs it, so that the
+// loads run under the previous step's products), put() writes it.  Rows >= n are not read (the last row stands in); rows whose bit of `bits` is 0 and
+// dims >= D become zeros: a masked row may hold anything, also NaN, and must not reach a product.  Row strides fit 22 bits, so a lane's place in a
+// tile is a 32-bit offset from a scalar address.
+template <typename T, int DP> struct AtTileIn {
+    static constexpr int CH = DP / 8, N = DP / 32;
+    const T* base;
+    long long stride;
+    int n, off[N];
+    bool in;                     // the lane's dims exist
+    V8<T> x[N];
+    __device__ __forceinline__ AtTileIn(const T* base_, long long stride_, int n_, int D) : base(base_), stride(stride_), n(n_) {
+        const int c = (int)threadIdx.x % CH;
+        in = c * 8 < D;
 #pragma unroll
-    for (int t = 0; t < AT_TILE * CH / AT_BLOCK; ++t) {
-        const int e = t * AT_BLOCK + (int)threadIdx.x, r = e / CH, c = e % CH;
-        V8<T> x = {};
-        if (((bits >> r) & 1) && c * 8 < D) x = *(const V8<T>*)(src + (long long)(r0 + r) * stride + c * 8);
-        *(V8<T>*)at_at<T, DP>(tile, r, c) = x;
+        for (int t = 0; t < N; ++t) off[t] = row(t) * (int)stride + (in ? c * 8 : 0);
     }
+    static __device__ __forceinline__ int row(int t) { return (t * AT_BLOCK + (int)threadIdx.x) / CH; }
+    __device__ __forceinline__ void fetch(int r0) {
+        const T* at = base + (long long)r0 * stride;
+        const int over = r0 - (n - 1);
+#pragma unroll
+        for (int t = 0; t < N; ++t) x[t] = *(const V8<T>*)(at + (off[t] - __mul24(max(0, over + row(t)), (int)stride)));
+    }
+    __device__ __forceinline__ void put(T* tile, u64 bits, bool whole) const {
+        const int c = (int)threadIdx.x % CH;
+        if (bits == ~0ull && whole) {
+#pragma unroll
+            for (int t = 0; t < N; ++t) *(V8<T>*)at_at<T, DP>(tile, row(t), c) = x[t];
+        } else {
+#pragma unroll
+            for (int t = 0; t < N; ++t) *(V8<T>*)at_at<T, DP>(tile, row(t), c) = in && ((bits >> row(t)) & 1) ? x[t] : V8<T>{};
+        }
+    }
+};
+__device__ __forceinline__ u64 read_lane(u64 x, int lane) {
+    return ((u64)(u32)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32) | (u32)__builtin_amdgcn_readlane((int)x, lane);
 }
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 // A fragment: rows row0 + l % 32, dims 16 s + 8 (l / 32) + j
 template <typename T, int DP> __device__ __forceinline__ V8<T> at_rows(T* tile, int row0, int s) {
     const int l = threadIdx.x & 63;
@@ -79,11 +113,26 @@ template <typename T, int DP> __device__ __forceinline__ V8<T> at_rows(T* tile, 
 }
 // A fragment of the transposed tile: row = dim 32 dt + l % 32, places j = tile rows row0 + 16 m + 8 (j / 4) + 4 (l / 32) + j % 4: the rows
 // that half l / 32 of a result tile holds in its registers 8 m + j
+// (16-bit types: two transposing reads of 4 rows x 16 dims per group of 16 lanes; lane i of a group points at dims 4 (i % 4).. of row i / 4 and
+// receives dim i of the 4 rows)
 template <typename T, int DP> __device__ __forceinline__ V8<T> at_cols(T* tile, int row0, int m, int dt) {
-    const int l = threadIdx.x & 63, d = 32 * dt + (l & 31);
+    const int l = threadIdx.x & 63;
     V8<T> x;
+    if constexpr (sizeof(T) == 2) {
+        const int d = 32 * dt + 16 * ((l >> 4) & 1) + 4 * (l & 3);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = at_at<T, DP>(tile, row0 + 16 * m + 8 * (j >> 2) + 4 * (l >> 5) + (j & 3), d >> 3)[d & 7];
+        for (int jj = 0; jj < 2; ++jj) {
+            T* from = at_at<T, DP>(tile, row0 + 16 * m + 8 * jj + 4 * (l >> 5) + ((l & 15) >> 2), d >> 3) + (d & 7);
+            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from);
+            const V4<T> y = __builtin_bit_cast(V4<T>, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * jj + j] = y[j];
+        }
+    } else {
+        const int d = 32 * dt + (l & 31);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = at_at<T, DP>(tile, row0 + 16 * m + 8 * (j >> 2) + 4 * (l >> 5) + (j & 3), d >> 3)[d & 7];
+    }
     return x;
 }
 // B fragment straight from memory: column = row `row` of the matrix, dims 16 s + 8 half + j
@@ -123,60 +172,116 @@ template <typename T, int DP> __device__ __forceinline__ void at_store(T* row, c
         }
 }
 
-// visibility of keys [k0, k0 + 64) as bits: the key mask and the end of the keys
-__device__ __forceinline__ u64 at_word(const AttnParams& p, int b, int k0, int end) {
-    const int k = k0 + (int)(threadIdx.x & 63);
-    bool on = k < end;
-    if (on && p.mask) on = p.mask[(long long)b * p.mask_b + k] != 0;
-    return __ballot(on);
+// Visibility of the 4096 keys from `base`: lane t gets the 64 bits of tile t (key mask, and keys < end).  A lane packs its whole tile from eight
+// 8-byte loads; the tile that `end` cuts is read a byte per lane.
+__device__ __forceinline__ u64 at_words(const AttnParams& p, int b, int base, int end) {
+    const int l = threadIdx.x & 63, n = end - base, mine = n - l * AT_TILE;        // keys left from this lane's tile on
+    u64 w = mine >= 64 ? ~0ull : (mine > 0 ? (1ull << mine) - 1 : 0ull);
+    if (p.mask) {
+        const unsigned char* m = p.mask + (long long)b * p.mask_b + base;
+        if (mine >= 64) {
+            w = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                u64 x;
+                __builtin_memcpy(&x, m + l * AT_TILE + j * 8, 8);
+                x = ((((x & 0x7f7f7f7f7f7f7f7full) + 0x7f7f7f7f7f7f7f7full) | x) >> 7) & 0x0101010101010101ull;   // 1 for every byte that is not 0
+                w |= ((x * 0x0102040810204080ull) >> 56) << (8 * j);
+            }
+        }
+        if (n < 64 * AT_TILE && (n & 63)) {
+            const int at = (n & ~63) + l;
+            const u64 cut = __ballot(at < n && m[at < n ? at : 0] != 0);
+            if (l == n >> 6) w = cut;
+        }
+    }
+    return w;
 }
 
-// bias of this lane's 16 elements of a 32 x 32 tile whose first key is k0 (queries in lanes): s2 = s * c + bias, masked places -inf.
-// sign = +1: the lane's column is a query at position `col`, rows are keys; sign = -1: the column is a key, rows are queries.
+// hidden keys of a 32 x 32 tile (bit per row) -> -inf
+__device__ __forceinline__ void at_hide(f32x16& s, u32 seen) {
+    seen >>= 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (!((seen >> crow(i, 0)) & 1)) s[i] = -__builtin_inff();
+}
+
+// Runs `step(k0, bits)` for every tile of 64 keys in [0, end) that shows any key, with the tile's K and V in LDS; by the whole block.
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void at_for_tiles(const AttnParams& p, int b, int h, int end, T* kt, T* vt, F&& step) {
+    AtTileIn<T, DP> kr((const T*)p.k + b * p.k_b + h * p.k_h, p.k_l, end, p.D), vr((const T*)p.v + b * p.v_b + h * p.v_h, p.v_l, end, p.D);
+    const bool whole = p.D == DP;
+    for (int base = 0; base < end; base += 64 * AT_TILE) {
+        const u64 words = at_words(p, b, base, end);
+        u64 left = __ballot(words != 0);                                   // the same in every wave
+        if (!left) continue;
+        int t = __builtin_ctzll(left);
+        kr.fetch(base + t * AT_TILE);
+        vr.fetch(base + t * AT_TILE);
+        while (true) {
+            const int k0 = base + t * AT_TILE;
+            const u64 bits = read_lane(words, t);
+            left &= left - 1;
+            __syncthreads();                                               // (the last step's readers are done)
+            kr.put(kt, bits, whole);
+            vr.put(vt, bits, whole);
+            __syncthreads();
+            if (left) {
+                t = __builtin_ctzll(left);
+                kr.fetch(base + t * AT_TILE);
+                vr.fetch(base + t * AT_TILE);
+            }
+            step(k0, bits);
+            if (!left) break;
+        }
+    }
+}
+
+// The bias table in LDS: distances -(sat + 63) .. sat + 63, so that a 32 x 32 tile which holds any distance inside (-sat, sat) stays inside it and
+// is read without clamping, at fixed offsets from one address per lane.
+#define AT_EDGE 63
+__device__ __forceinline__ int at_lut_size(int sat) { return 2 * (sat + AT_EDGE) + 1; }
+__device__ __forceinline__ void at_lut(const AttnParams& p, float* lut, int h) {
+    for (int i = threadIdx.x; i < at_lut_size(p.sat); i += AT_BLOCK)
+        lut[i] = p.table[(long long)attn_bucket(p, i - p.sat - AT_EDGE) * p.H + h] * LOG2E;
+}
+// s2 = s * c + bias for this lane's 16 elements of a 32 x 32 tile, places behind the query -inf when causal.
+// SIGN = +1: the lane's column is a query at position `col`, rows are keys from row0; -1: the column is a key, rows are query positions from row0.
 template <int SIGN>
-__device__ __forceinline__ void at_bias(f32x16& s, const float* lut, int sat, float c, int row0, int col, int col_lo, int col_hi, bool causal) {
+__device__ __forceinline__ void at_bias(f32x16& s, const float* lut, int sat, float c, int row0, int col, int col_lo, bool causal) {
     const int half = (threadIdx.x & 63) >> 5;
-    const int lo = SIGN > 0 ? row0 - col_hi : col_lo - (row0 + 31), hi = SIGN > 0 ? row0 + 31 - col_lo : col_hi - row0;   // key - query over the tile
+    const int lo = SIGN > 0 ? row0 - col_lo - 31 : col_lo - row0 - 31, hi = lo + 62;      // key - query over the tile
     if (lo >= sat || hi <= -sat) {
-        const float add = lut[lo >= sat ? 2 * sat : 0];
+        const float add = lut[lo >= sat ? 2 * (sat + AT_EDGE) : 0];
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], c, add);
     } else {
+        const float* at = lut + (SIGN > 0 ? row0 + 4 * half - col : col - row0 - 4 * half) + sat + AT_EDGE;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int r = row0 + crow(i, half);
-            int d = SIGN > 0 ? r - col : col - r;
-            d = d < -sat ? -sat : (d > sat ? sat : d);
-            s[i] = __builtin_fmaf(s[i], c, lut[d + sat]);
-        }
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], c, at[SIGN * crow(i, 0)]);
     }
     if (causal && hi > 0) {
+        const int edge = SIGN > 0 ? col - row0 - 4 * half : row0 + 4 * half - col;         // the last visible row / minus the first
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int r = row0 + crow(i, half);
-            if ((SIGN > 0 ? r - col : col - r) > 0) s[i] = -__builtin_inff();
-        }
+        for (int i = 0; i < 16; ++i)
+            if (SIGN > 0 ? crow(i, 0) > edge : crow(i, 0) + edge < 0) s[i] = -__builtin_inff();
     }
-}
-__device__ __forceinline__ void at_lut(const AttnParams& p, float* lut, int h) {
-    for (int i = threadIdx.x; i <= 2 * p.sat; i += AT_BLOCK) lut[i] = p.table[(long long)attn_bucket(p, i - p.sat) * p.H + h] * LOG2E;
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // KEEP (training, 16-bit types): D = <dO, O> of the backward pass enters the bias table's fp32 gradient, a difference of large sums.  P V takes
 // P in two parts (value and what its rounding dropped, error u^2) and out_lo keeps what the output's rounding dropped.
 template <typename T, int DP, bool KEEP>
-__global__ __launch_bounds__(AT_BLOCK) void mfar_attn_forward_kernel(const AttnParams p) {
+__global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_attn_forward_kernel(const AttnParams p) {
     extern __shared__ __align__(16) unsigned char at_lds[];
     T* kt = (T*)at_lds;
     T* vt = kt + AT_TILE * DP;
-    u64* words = (u64*)(vt + AT_TILE * DP);
-    float* lut = (float*)(words + 64);
-    const int b = blockIdx.z, h = blockIdx.y, wave = threadIdx.x >> 6, l = threadIdx.x & 63, half = l >> 5;
+    float* lut = (float*)(vt + AT_TILE * DP);
+    const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5;
     const int start = at_start(p, b);
     const int q = blockIdx.x * AT_COLS + wave * 32 + (l & 31);
     const bool live = q < p.Lq;
-    const int col = start + q, col_lo = start + (int)blockIdx.x * AT_COLS + wave * 32, col_hi = col_lo + 31;
+    const int col = start + q, col_lo = start + (int)blockIdx.x * AT_COLS + wave * 32;
     int end = p.Lk;
     if (p.causal) {
         const int last = start + min(p.Lq, ((int)blockIdx.x + 1) * AT_COLS);      // one past the last query's position
@@ -190,67 +295,43 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_forward_kernel(const AttnP
     f32x16 acc[DP / 32] = {};
     float m = -__builtin_inff(), sum = 0.0f;
     const float c = p.scale * LOG2E;
-    const T* kb = (const T*)p.k + b * p.k_b + h * p.k_h;
-    const T* vb = (const T*)p.v + b * p.v_b + h * p.v_h;
-    for (int k0 = 0; k0 < end; k0 += AT_TILE) {
-        const int tile = k0 / AT_TILE;
-        if ((tile & 63) == 0) {                                            // the visibility of the next 64 tiles
-            __syncthreads();
-            for (int t = wave; t < 64; t += 4) {
-                const u64 w = at_word(p, b, k0 + t * AT_TILE, end);
-                if (l == 0) words[t] = w;
-            }
-            __syncthreads();
-        }
-        const u64 bits = words[tile & 63];
-        if (!bits) continue;                                               // (the same for the whole block)
-        __syncthreads();
-        at_stage<T, DP>(kt, kb, p.k_l, k0, bits, p.D);
-        at_stage<T, DP>(vt, vb, p.v_l, k0, bits, p.D);
-        __syncthreads();
-        f32x16 s[2];
-        float top = m;
+    at_for_tiles<T, DP>(p, b, h, end, kt, vt, [&](int k0, u64 bits) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            s[t] = f32x16{};
+            const u32 seen = (u32)(bits >> (32 * t));
+            f32x16 s = {};
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) s[t] = mma(at_rows<T, DP>(kt, 32 * t, d), qf[d], s[t]);
-            at_bias<1>(s[t], lut, p.sat, c, k0 + 32 * t, col, col_lo, col_hi, p.causal != 0);
-            if (bits != ~0ull) {
-                const u32 mine = (u32)(bits >> (32 * t)) >> (4 * half);
+            for (int d = 0; d < DP / 16; ++d) s = mma(at_rows<T, DP>(kt, 32 * t, d), qf[d], s);
+            at_bias<1>(s, lut, p.sat, c, k0 + 32 * t, col, col_lo, p.causal != 0);
+            if (seen != ~0u) at_hide(s, seen);
+            float top = -__builtin_inff();
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!((mine >> crow(i, 0)) & 1)) s[t][i] = -__builtin_inff();
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+            top = max_halves(top);
+            if (__any(top > m + AT_SLACK)) {                                // (m = -inf at first: any number is over it)
+                const float up = fmaxf(top, m), keep = up == -__builtin_inff() ? 1.0f : exp2_fast(m - up);
+                m = up;
+                sum *= keep;
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= keep;
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-        }
-        top = fmaxf(top, swap_halves(top));
-        const float base = top == -__builtin_inff() ? 0.0f : top;           // nothing visible so far: exp2(-inf - 0) = 0
-        const float keep = exp2_fast(m - base);
-        m = top;
-        sum *= keep;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
+            const float base = m == -__builtin_inff() ? 0.0f : m;           // nothing visible so far: exp2(-inf - 0) = 0
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[t][i] = exp2_fast(s[t][i] - base);
-                sum += s[t][i];
+                s[i] = exp2_fast(s[i] - base);
+                sum += s[i];
             }
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) {
-            acc[dt] *= keep;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const V8<T> vf = at_cols<T, DP>(vt, 32 * t, g, dt);
-                    acc[dt] = mma(vf, at_pack<T>(s[t], g), acc[dt]);
-                    if (KEEP) acc[dt] = mma(vf, at_pack_lo<T>(s[t], g), acc[dt]);
+                    acc[dt] = mma(vf, at_pack<T>(s, g), acc[dt]);
+                    if (KEEP) acc[dt] = mma(vf, at_pack_lo<T>(s, g), acc[dt]);
                 }
         }
-    }
-    sum += swap_halves(sum);
+    });
+    sum = sum_halves(sum);
     if (!live) return;
     const float f = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);    // a row without keys: zeros; NaN stays NaN
     const long long row = ((long long)b * p.Lq + q) * p.H + h;
@@ -265,27 +346,51 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_forward_kernel(const AttnP
     if (p.lse && half == 0) p.lse[((long long)b * p.H + h) * p.Lq + q] = sum == 0.0f ? -__builtin_inff() : m + __log2f(sum);
 }
 
+// Sums along the diagonals of a 32 x 32 tile (lanes: queries, registers: keys), added to sums[key - query]; by one wave, in memory of its own.
+// The tile goes through LDS: lane m of either half reads the 16 elements of its half's rows with (row - column) % 32 = m.  Those with row >= m lie on
+// diagonal m, the others on m - 32; half 0 then adds to the former, half 1 to the latter: 64 different places, no atomics (LDS float atomics
+// took 205 cycles per wave here, 16 of them per tile).
+__device__ __forceinline__ void at_diagonals(const f32x16& s, float* skew, float* sums) {
+    const int l = threadIdx.x & 63, half = l >> 5, m = l & 31;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) skew[(crow(i, 0) + 4 * half) * 32 + m] = s[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float all = 0.0f, on = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int r = 16 * half + j;
+        const float x = skew[r * 32 + ((r - m) & 31)];
+        all += x;
+        on += r >= m ? x : 0.0f;
+    }
+    const float off = sum_halves(all - on);
+    on = sum_halves(on);
+    sums[half ? m - 32 : m] += half ? off : on;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---- backward: dQ, the bias gradient, D ---------------------------------------------------------------------------------------------------
 template <typename T, int DP>
-__global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dq_kernel(const AttnParams p) {
+__global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_attn_dq_kernel(const AttnParams p) {
     extern __shared__ __align__(16) unsigned char at_lds[];
     T* kt = (T*)at_lds;
     T* vt = kt + AT_TILE * DP;
-    u64* words = (u64*)(vt + AT_TILE * DP);
-    float* lut = (float*)(words + 64);
-    const int n_lut = 2 * p.sat + 1;
-    float* hist = lut + n_lut;                                             // [4 waves][2 halves][n_lut]: a lane meets no other at an address
-    const int b = blockIdx.z, h = blockIdx.y, wave = threadIdx.x >> 6, l = threadIdx.x & 63, half = l >> 5;
+    float* lut = (float*)(vt + AT_TILE * DP);
+    const int n_lut = at_lut_size(p.sat);
+    float* hist = lut + n_lut;                                             // [4 waves][n_lut] sums of dS by distance
+    float* skew = hist + 4 * n_lut;                                        // [4 waves][32][32]
+    const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5;
     const int start = at_start(p, b);
     const int q = blockIdx.x * AT_COLS + wave * 32 + (l & 31);
     const bool live = q < p.Lq;
-    const int col = start + q, col_lo = start + (int)blockIdx.x * AT_COLS + wave * 32, col_hi = col_lo + 31;
+    const int col = start + q, col_lo = start + (int)blockIdx.x * AT_COLS + wave * 32;
     int end = p.Lk;
     if (p.causal) end = min(end, max(start + min(p.Lq, ((int)blockIdx.x + 1) * AT_COLS), 0));
     at_lut(p, lut, h);
     if (p.dpart)
-        for (int i = threadIdx.x; i < 8 * n_lut; i += AT_BLOCK) hist[i] = 0.0f;
-    float* mine_hist = hist + (wave * 2 + half) * n_lut;
+        for (int i = threadIdx.x; i < 4 * n_lut; i += AT_BLOCK) hist[i] = 0.0f;
     const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
     const T* grow = (const T*)p.dout + b * p.do_b + (long long)q * p.do_l + h * p.do_h;
     const long long orow = (((long long)b * p.Lq + q) * p.H + h) * p.D;
@@ -299,7 +404,7 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dq_kernel(const AttnParams
 #pragma unroll
         for (int j = 0; j < 8; ++j) dsum = __builtin_fmaf((float)gf[s][j], (float)o[j] + (float)lo[j], dsum);
     }
-    dsum += swap_halves(dsum);
+    dsum = sum_halves(dsum);
     const long long srow = ((long long)b * p.H + h) * p.Lq + q;
     float lse = live ? p.lse[srow] : 0.0f;
     if (!live || lse == -__builtin_inff()) lse = __builtin_inff();          // no keys: P = exp2(-inf) = 0 everywhere
@@ -307,24 +412,7 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dq_kernel(const AttnParams
     f32x16 acc[DP / 32] = {};
     float far_lo = 0.0f, far_hi = 0.0f;
     const float c = p.scale * LOG2E;
-    const T* kb = (const T*)p.k + b * p.k_b + h * p.k_h;
-    const T* vb = (const T*)p.v + b * p.v_b + h * p.v_h;
-    for (int k0 = 0; k0 < end; k0 += AT_TILE) {
-        const int tile = k0 / AT_TILE;
-        if ((tile & 63) == 0) {
-            __syncthreads();
-            for (int t = wave; t < 64; t += 4) {
-                const u64 w = at_word(p, b, k0 + t * AT_TILE, end);
-                if (l == 0) words[t] = w;
-            }
-            __syncthreads();
-        }
-        const u64 bits = words[tile & 63];
-        if (!bits) continue;
-        __syncthreads();
-        at_stage<T, DP>(kt, kb, p.k_l, k0, bits, p.D);
-        at_stage<T, DP>(vt, vb, p.v_l, k0, bits, p.D);
-        __syncthreads();
+    at_for_tiles<T, DP>(p, b, h, end, kt, vt, [&](int k0, u64 bits) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int row0 = k0 + 32 * t;
@@ -334,29 +422,20 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dq_kernel(const AttnParams
                 s = mma(at_rows<T, DP>(kt, 32 * t, d), qf[d], s);
                 dp = mma(at_rows<T, DP>(vt, 32 * t, d), gf[d], dp);
             }
-            at_bias<1>(s, lut, p.sat, c, row0, col, col_lo, col_hi, p.causal != 0);
-            const u32 mine = (u32)(bits >> (32 * t)) >> (4 * half);
+            at_bias<1>(s, lut, p.sat, c, row0, col, col_lo, p.causal != 0);
+            const u32 shown = (u32)(bits >> (32 * t));
+            if (shown != ~0u) at_hide(s, shown);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float pr = exp2_fast(s[i] - lse);
-                s[i] = ((mine >> crow(i, 0)) & 1) ? pr * (dp[i] - dsum) : 0.0f;
-            }
+            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i] - lse) * (dp[i] - dsum);
             if (p.dpart) {
-                if (row0 - col_hi >= p.sat) {
+                if (row0 - col_lo - 31 >= p.sat) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) far_hi += s[i];
                 } else if (row0 + 31 - col_lo <= -p.sat) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) far_lo += s[i];
                 } else {
-                    // 32 lanes of a half hold 32 neighbouring distances: one address each; distances beyond sat go to the lane's own sums
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int d = row0 + crow(i, half) - col;
-                        if (d >= p.sat) far_hi += s[i];
-                        else if (d <= -p.sat) far_lo += s[i];
-                        else mine_hist[d + p.sat] += s[i];
-                    }
+                    at_diagonals(s, skew + wave * 1024, hist + wave * n_lut + (row0 - col_lo) + p.sat + AT_EDGE);
                 }
             }
 #pragma unroll
@@ -364,7 +443,7 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dq_kernel(const AttnParams
 #pragma unroll
                 for (int g = 0; g < 2; ++g) acc[dt] = mma(at_cols<T, DP>(kt, 32 * t, g, dt), at_pack<T>(s, g), acc[dt]);
         }
-    }
+    });
     if (live) at_store<T, DP>((T*)p.dq + orow, acc, p.scale, p.D);
     if (p.dpart) {
         for (int o = 1; o < 64; o <<= 1) {
@@ -373,16 +452,26 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dq_kernel(const AttnParams
         }
         __syncthreads();
         if (l == 0) {
-            hist[wave * 2 * n_lut] = far_lo;                               // places 0 and 2 sat of the wave's first row
-            hist[wave * 2 * n_lut + 2 * p.sat] += far_hi;                  // (sat = 0 cannot be: the first bucket holds distance 0 alone)
+            hist[wave * n_lut] += far_lo;                                  // the outermost distances: both in a last bucket
+            hist[wave * n_lut + n_lut - 1] += far_hi;
         }
         __syncthreads();
+        for (int i = threadIdx.x; i < n_lut; i += AT_BLOCK) {
+            float t = 0.0f;
+            for (int w = 0; w < 4; ++w) t += hist[w * n_lut + i];
+            hist[i] = t;
+        }
+        __syncthreads();
+        // a bucket holds the distances [lo, hi) of one side
         float* to = p.dpart + ((long long)(b * gridDim.x + blockIdx.x) * p.H + h) * p.n_buckets;
         for (int n = threadIdx.x; n < p.n_buckets; n += AT_BLOCK) {
+            const bool ahead = n >= p.n_side;
+            const int m = n - (ahead ? p.n_side : 0), top = p.sat + AT_EDGE + 1;
+            int lo = m <= p.each ? m : p.borders[m - p.each - 1];
+            const int hi = m < p.each ? m + 1 : (m == p.n_side - 1 ? top : p.borders[m - p.each]);
+            if (ahead && lo == 0) lo = 1;                                  // distance 0 counts as behind
             float t = 0.0f;
-            for (int i = 0; i < n_lut; ++i)
-                if (attn_bucket(p, i - p.sat) == n)
-                    for (int w = 0; w < 8; ++w) t += hist[w * n_lut + i];
+            for (int d = lo; d < hi; ++d) t += hist[(ahead ? d : -d) + p.sat + AT_EDGE];
             to[n] = t;
         }
     }
@@ -404,18 +493,18 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dtable_kernel(const float*
 
 // ---- backward: dK, dV (keys in lanes) -------------------------------------------------------------------------------------------------------
 template <typename T, int DP>
-__global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dkv_kernel(const AttnParams p) {
+__global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_attn_dkv_kernel(const AttnParams p) {
     extern __shared__ __align__(16) unsigned char at_lds[];
     T* qt = (T*)at_lds;
     T* gt = qt + AT_TILE * DP;
     float* rows = (float*)(gt + AT_TILE * DP);                             // [2][AT_TILE]: log2-sum, D
     float* lut = rows + 2 * AT_TILE;
-    const int b = blockIdx.z, h = blockIdx.y, wave = threadIdx.x >> 6, l = threadIdx.x & 63, half = l >> 5;
+    const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5;
     const int start = at_start(p, b);
     const int key0 = blockIdx.x * AT_COLS, key = key0 + wave * 32 + (l & 31);
     const bool live = key < p.Lk;
     const bool seen = live && (!p.mask || p.mask[(long long)b * p.mask_b + key] != 0);
-    const int col_lo = key0 + wave * 32, col_hi = col_lo + 31;
+    const int col_lo = key0 + wave * 32;
     at_lut(p, lut, h);
     const T* krow = (const T*)p.k + b * p.k_b + (long long)key * p.k_l + h * p.k_h;
     const T* vrow = (const T*)p.v + b * p.v_b + (long long)key * p.v_l + h * p.v_h;
@@ -433,19 +522,28 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dkv_kernel(const AttnParam
     int first = p.causal ? max(0, key0 - start) : 0;                       // the first query that sees the block's first key
     const bool any = __syncthreads_or(seen);                               // (also the barrier behind at_lut)
     if (!any) first = p.Lq;
-    for (int q0 = first / AT_TILE * AT_TILE; q0 < p.Lq; q0 += AT_TILE) {
-        const int n = min(AT_TILE, p.Lq - q0);
-        const u64 bits = n == 64 ? ~0ull : ((1ull << n) - 1);
+    first = first / AT_TILE * AT_TILE;
+    AtTileIn<T, DP> qr(qb, p.q_l, p.Lq, p.D), gr(gb, p.do_l, p.Lq, p.D);
+    if (first < p.Lq) {
+        qr.fetch(first);
+        gr.fetch(first);
+    }
+    for (int q0 = first; q0 < p.Lq; q0 += AT_TILE) {
         __syncthreads();
-        at_stage<T, DP>(qt, qb, p.q_l, q0, bits, p.D);
-        at_stage<T, DP>(gt, gb, p.do_l, q0, bits, p.D);
+        const u64 bits = q0 + AT_TILE <= p.Lq ? ~0ull : (1ull << (p.Lq - q0)) - 1;
+        qr.put(qt, bits, p.D == DP);
+        gr.put(gt, bits, p.D == DP);
         if (threadIdx.x < AT_TILE) {
-            const bool in = (int)threadIdx.x < n;
+            const bool in = q0 + (int)threadIdx.x < p.Lq;
             const float e = in ? p.lse[srow + q0 + threadIdx.x] : -__builtin_inff();
             rows[threadIdx.x] = e == -__builtin_inff() ? __builtin_inff() : e;
             rows[AT_TILE + threadIdx.x] = in ? p.drow[srow + q0 + threadIdx.x] : 0.0f;
         }
         __syncthreads();
+        if (q0 + AT_TILE < p.Lq) {
+            qr.fetch(q0 + AT_TILE);
+            gr.fetch(q0 + AT_TILE);
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x16 s = {}, dp = {};
@@ -454,13 +552,12 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dkv_kernel(const AttnParam
                 s = mma(at_rows<T, DP>(qt, 32 * t, d), kf[d], s);
                 dp = mma(at_rows<T, DP>(gt, 32 * t, d), vf[d], dp);
             }
-            at_bias<-1>(s, lut, p.sat, c, start + q0 + 32 * t, key, col_lo, col_hi, p.causal != 0);
+            at_bias<-1>(s, lut, p.sat, c, start + q0 + 32 * t, key, col_lo, p.causal != 0);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = 32 * t + crow(i, half);
-                const float pr = seen ? exp2_fast(s[i] - rows[r]) : 0.0f;
-                s[i] = pr;
-                dp[i] = seen ? pr * (dp[i] - rows[AT_TILE + r]) : 0.0f;
+                s[i] = exp2_fast(s[i] - rows[r]);
+                dp[i] = s[i] * (dp[i] - rows[AT_TILE + r]);
             }
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
@@ -472,6 +569,10 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dkv_kernel(const AttnParam
         }
     }
     if (!live) return;
+    if (!seen) {                                                           // a hidden key's column met no other: its sums are dropped here
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) dk[dt] = f32x16{}, dv[dt] = f32x16{};
+    }
     const long long row = (((long long)b * p.Lk + key) * p.H + h) * p.D;
     at_store<T, DP>((T*)p.dk + row, dk, p.scale, p.D);
     at_store<T, DP>((T*)p.dv + row, dv, 1.0f, p.D);

@@ -91,6 +91,8 @@ int check_attention(const mfar_attention* a, bool backward) {
     const int64_t strides[] = {a->q_b, a->q_l, a->q_h, a->k_b, a->k_l, a->k_h, a->v_b, a->v_l, a->v_h};
     for (int64_t s : strides)
         if (s * es % 16) return bad("strides must be multiples of 16 bytes");
+    for (int64_t s : {a->q_l, a->k_l, a->v_l, backward ? a->do_l : 0})
+        if (s < 0 || s > AT_MAX_STRIDE) return bad("row strides must be 0..2^22 elements");
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) || !aligned16(a->out_lo)) return bad("tensors must be 16-byte aligned");
     if (backward) {
         if (!a->dout || !a->dq || !a->lse || (a->Lk && (!a->dk || !a->dv))) return bad("NULL gradient or lse");
@@ -114,10 +116,10 @@ AttnParams attention_params(const mfar_attention* a) {
     return p;
 }
 int64_t drow_bytes(const mfar_attention* a) { return ((int64_t)a->B * a->H * a->Lq * 4 + 15) / 16 * 16; }
-size_t lut_bytes(const AttnParams& p) { return (size_t)(2 * p.sat + 1) * 4; }
+size_t lut_bytes(const AttnParams& p) { return (size_t)(2 * (p.sat + AT_EDGE) + 1) * 4; }
 
 template <typename T, int DP> int attention_forward(const AttnParams& p, hipStream_t st) {
-    const size_t lds = 2ull * AT_TILE * DP * sizeof(T) + 64 * 8 + lut_bytes(p);
+    const size_t lds = 2ull * AT_TILE * DP * sizeof(T) + lut_bytes(p);
     const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
     if constexpr (sizeof(T) == 2)
         if (p.out_lo) return launch<mfar_attn_forward_kernel<T, DP, true>>("mfar_attn_forward_kernel", grid, lds, st, p);
@@ -126,7 +128,7 @@ template <typename T, int DP> int attention_forward(const AttnParams& p, hipStre
 template <typename T, int DP> int attention_backward(const AttnParams& p, float* dtable, hipStream_t st) {
     const size_t tiles = 2ull * AT_TILE * DP * sizeof(T);
     const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
-    int rc = launch<mfar_attn_dq_kernel<T, DP>>("mfar_attn_dq_kernel", grid, tiles + 64 * 8 + lut_bytes(p) * (p.dpart ? 9 : 1), st, p);
+    int rc = launch<mfar_attn_dq_kernel<T, DP>>("mfar_attn_dq_kernel", grid, tiles + lut_bytes(p) * (p.dpart ? 5 : 1) + (p.dpart ? 4 * 1024 * 4 : 0), st, p);
     if (rc != MFAR_OK) return rc;
     if (p.Lk) {
         rc = launch<mfar_attn_dkv_kernel<T, DP>>("mfar_attn_dkv_kernel", dim3(cdiv(p.Lk, AT_COLS), p.H, p.B), tiles + 2 * AT_TILE * 4 + lut_bytes(p), st, p);

@@ -15,6 +15,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32;
 typedef unsigned long long u64;
 typedef u32 u32x4 __attribute__((ext_vector_type(4)));
@@ -36,7 +37,22 @@ __device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
     return c;
 }
 
-__device__ __forceinline__ float swap_halves(float x) { return __shfl_xor(x, 32); }
+// the two halves' values of a column, in either half (v_permlane32_swap: no LDS round trip)
+__device__ __forceinline__ void both_halves(float x, float& a, float& b) {
+    typedef u32 u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    a = __uint_as_float(y[0]), b = __uint_as_float(y[1]);
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    float a, b;
+    both_halves(x, a, b);
+    return a + b;
+}
+__device__ __forceinline__ float max_halves(float x) {
+    float a, b;
+    both_halves(x, a, b);
+    return fmaxf(a, b);
+}
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, below 2^-126 flushed to zero
 #define LOG2E 1.44269504088896341f
 #define LN2 0.693147180559945309f

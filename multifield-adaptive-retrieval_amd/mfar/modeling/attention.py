@@ -51,6 +51,7 @@ def _strided(x: torch.Tensor) -> torch.Tensor:
     es = x.element_size()
     ok = x.stride(3) == 1 or x.size(3) == 1
     ok = ok and x.data_ptr() % 16 == 0 and all(x.stride(i) * es % 16 == 0 or x.size(i) == 1 for i in range(3))
+    ok = ok and (x.size(1) == 1 or x.stride(1) <= 2 ** 22)
     return x if ok else x.contiguous()
 
 
