@@ -268,6 +268,38 @@ __device__ __forceinline__ void at_bias(f32x16& s, const float* lut, int sat, fl
     }
 }
 
+// One 32 x 32 tile of scores into the running softmax: maximum m, this half's part of the sum, and O' += V' P' with the rows from row0 of vt.
+template <typename T, int DP, bool KEEP>
+__device__ __forceinline__ void at_softmax(f32x16& s, T* vt, int row0, float& m, float& sum, f32x16* acc) {
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+    top = max_halves(top);
+    if (__any(top > m + AT_SLACK)) {                                        // (m = -inf at first: any number is over it)
+        const float up = fmaxf(top, m), keep = up == -__builtin_inff() ? 1.0f : exp2_fast(m - up);
+        m = up;
+        sum *= keep;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= keep;
+    }
+    const float base = m == -__builtin_inff() ? 0.0f : m;                   // nothing visible so far: exp2(-inf - 0) = 0
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        s[i] = exp2_fast(s[i] - base);
+        sum += s[i];
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const V8<T> vf = at_cols<T, DP>(vt, row0, g, dt);
+            acc[dt] = mma(vf, at_pack<T>(s, g), acc[dt]);
+            if (KEEP) acc[dt] = mma(vf, at_pack_lo<T>(s, g), acc[dt]);
+        }
+}
+
+__device__ __forceinline__ float at_norm(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }   // no keys: zeros; NaN stays
+
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // KEEP (training, 16-bit types): D = <dO, O> of the backward pass enters the bias table's fp32 gradient, a difference of large sums.  P V takes
 // P in two parts (value and what its rounding dropped, error u^2) and out_lo keeps what the output's rounding dropped.
@@ -304,36 +336,12 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
             for (int d = 0; d < DP / 16; ++d) s = mma(at_rows<T, DP>(kt, 32 * t, d), qf[d], s);
             at_bias<1>(s, lut, p.sat, c, k0 + 32 * t, col, col_lo, p.causal != 0);
             if (seen != ~0u) at_hide(s, seen);
-            float top = -__builtin_inff();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
-            top = max_halves(top);
-            if (__any(top > m + AT_SLACK)) {                                // (m = -inf at first: any number is over it)
-                const float up = fmaxf(top, m), keep = up == -__builtin_inff() ? 1.0f : exp2_fast(m - up);
-                m = up;
-                sum *= keep;
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= keep;
-            }
-            const float base = m == -__builtin_inff() ? 0.0f : m;           // nothing visible so far: exp2(-inf - 0) = 0
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[i] = exp2_fast(s[i] - base);
-                sum += s[i];
-            }
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const V8<T> vf = at_cols<T, DP>(vt, 32 * t, g, dt);
-                    acc[dt] = mma(vf, at_pack<T>(s, g), acc[dt]);
-                    if (KEEP) acc[dt] = mma(vf, at_pack_lo<T>(s, g), acc[dt]);
-                }
+            at_softmax<T, DP, KEEP>(s, vt, 32 * t, m, sum, acc);
         }
     });
     sum = sum_halves(sum);
     if (!live) return;
-    const float f = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);    // a row without keys: zeros; NaN stays NaN
+    const float f = at_norm(sum);
     const long long row = ((long long)b * p.Lq + q) * p.H + h;
     at_store<T, DP>((T*)p.out + row * p.D, acc, f, p.D);
     if (KEEP) {
@@ -344,6 +352,151 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
         at_store<T, DP>((T*)p.out_lo + row * p.D, acc, 1.0f, p.D);
     }
     if (p.lse && half == 0) p.lse[((long long)b * p.H + h) * p.Lq + q] = sum == 0.0f ? -__builtin_inff() : m + __log2f(sum);
+}
+
+// ---- forward, up to 32 queries (short texts, a decoder's next token): the work is in the keys ------------------------------------------------
+// Tiles of 32 keys go to the waves in turn, 4 waves a block and `splits` blocks per (batch, head): K straight into fragments, V through LDS of the
+// wave's own, no barrier in the loop, the next tile's loads in flight.  The waves' partial softmaxes are joined in LDS, the blocks' in a second
+// launch, both in a fixed order.  Bound by reading K and V.
+struct AttnSplit {
+    float *o, *ml;               // [rows, splits, D], [rows, splits, 2] (maximum, sum); row = (batch * Lq + query) * H + head
+    int splits;
+};
+template <typename T> __device__ __forceinline__ void at_write(const AttnParams& p, bool keep, long long at, float x) {
+    const T y = (T)x;
+    ((T*)p.out)[at] = y;
+    if (keep) ((T*)p.out_lo)[at] = (T)(x - (float)y);
+}
+
+template <typename T, int DP, bool KEEP>
+__global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_attn_few_kernel(const AttnParams p, const AttnSplit sp) {
+    extern __shared__ __align__(16) unsigned char at_lds[];
+    T* vt = (T*)at_lds + wave_index() * 32 * DP;
+    float* part = (float*)at_lds;                                          // [4 waves][DP][32], behind the loop
+    float* stat = part + 4 * DP * 32;                                      // [4 waves][2][32]
+    float* lut = stat + 4 * 64;
+    const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5, q = l & 31;
+    const int start = at_start(p, b);
+    const bool live = q < p.Lq;
+    const int col = start + q;
+    const int end = p.causal ? min(p.Lk, max(start + p.Lq, 0)) : p.Lk;
+    constexpr int CH = DP / 8, NV = DP / 16;                               // chunks a row; chunks of V a lane
+    const T* kb = (const T*)p.k + b * p.k_b + h * p.k_h;
+    const T* vb = (const T*)p.v + b * p.v_b + h * p.v_h;
+    const unsigned char* mask = p.mask ? p.mask + (long long)b * p.mask_b : nullptr;
+    const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
+    V8<T> qf[DP / 16], kf[DP / 16], vr[NV];
+    bool on = false;
+    const int step = sp.splits * 4 * 32;
+    int k0 = ((int)blockIdx.x * 4 + wave) * 32;
+    const bool vin = (l % CH) * 8 < p.D;
+    auto fetch = [&]() {
+        const int key = min(k0 + (l & 31), end - 1);
+        const T* row = kb + (long long)key * p.k_l;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) kf[s] = at_load<T>(row, true, s, p.D);
+#pragma unroll
+        for (int t = 0; t < NV; ++t) {
+            const int r = min(k0 + (t * 64 + l) / CH, end - 1);
+            vr[t] = *(const V8<T>*)(vb + (long long)r * p.v_l + (vin ? (l % CH) * 8 : 0));
+        }
+        on = k0 + (l & 31) < end && (!mask || mask[key] != 0);
+    };
+    if (k0 < end) fetch();
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) qf[s] = at_load<T>(qrow, live, s, p.D);
+    at_lut(p, lut, h);
+    __syncthreads();
+    f32x16 acc[DP / 32] = {};
+    float m = -__builtin_inff(), sum = 0.0f;
+    const float c = p.scale * LOG2E;
+    while (k0 < end) {
+        const u32 seen = (u32)__ballot(on);
+        const int row0 = k0;
+        f32x16 s = {};
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) s = mma(kf[d], qf[d], s);
+#pragma unroll
+        for (int t = 0; t < NV; ++t) {
+            const int r = (t * 64 + l) / CH;
+            *(V8<T>*)at_at<T, DP>(vt, r, l % CH) = vin && ((seen >> r) & 1) ? vr[t] : V8<T>{};
+        }
+        k0 += step;
+        if (k0 < end) fetch();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (seen) {
+            at_bias<1>(s, lut, p.sat, c, row0, col, start, p.causal != 0);
+            if (seen != ~0u) at_hide(s, seen);
+            at_softmax<T, DP, KEEP>(s, vt, 0, m, sum, acc);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    sum = sum_halves(sum);
+    __syncthreads();                                                       // (part lies where the V tiles were)
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(wave * DP + 32 * dt + crow(i, half)) * 32 + q] = acc[dt][i];
+    if (half == 0) {
+        stat[wave * 64 + q] = m;
+        stat[wave * 64 + 32 + q] = sum;
+    }
+    __syncthreads();
+    if (!live) return;
+    float f[4], all = 0.0f;
+    m = fmaxf(fmaxf(stat[q], stat[64 + q]), fmaxf(stat[128 + q], stat[192 + q]));
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = exp2_fast(stat[w * 64 + q] - base);
+        all += f[w] * stat[w * 64 + 32 + q];
+    }
+    const long long row = ((long long)b * p.Lq + q) * p.H + h;
+    const float norm = sp.splits == 1 ? at_norm(all) : 1.0f;
+    for (int d = threadIdx.x >> 5; d < p.D; d += 8) {
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) x += f[w] * part[(w * DP + d) * 32 + q];
+        if (sp.splits == 1) at_write<T>(p, KEEP, row * p.D + d, x * norm);
+        else sp.o[(row * sp.splits + blockIdx.x) * p.D + d] = x;
+    }
+    if (threadIdx.x < 32) {
+        if (sp.splits > 1) {
+            float* to = sp.ml + (row * sp.splits + blockIdx.x) * 2;
+            to[0] = m, to[1] = all;
+        } else if (p.lse) {
+            p.lse[((long long)b * p.H + h) * p.Lq + q] = all == 0.0f ? -__builtin_inff() : m + __log2f(all);
+        }
+    }
+}
+// joins the blocks of mfar_attn_few_kernel: one wave per row
+template <typename T, bool KEEP> __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_join_kernel(const AttnParams p, const AttnSplit sp) {
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (long long)p.B * p.Lq * p.H;
+    const int l = threadIdx.x & 63;
+    if (row >= rows) return;
+    const float* ml = sp.ml + row * sp.splits * 2;
+    float m = -__builtin_inff(), sum = 0.0f;
+    for (int s = 0; s < sp.splits; ++s) m = fmaxf(m, ml[2 * s]);
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+    float x[2] = {};
+    for (int s = 0; s < sp.splits; ++s) {
+        const float f = exp2_fast(ml[2 * s] - base);
+        sum += f * ml[2 * s + 1];
+        const float* o = sp.o + (row * sp.splits + s) * p.D;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (l + 64 * j < p.D) x[j] += f * o[l + 64 * j];
+    }
+    const float norm = at_norm(sum);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (l + 64 * j < p.D) at_write<T>(p, KEEP, row * p.D + l + 64 * j, x[j] * norm);
+    if (p.lse && l == 0) {
+        const long long h = row % p.H, q = row / p.H % p.Lq, b = row / p.H / p.Lq;
+        p.lse[(b * p.H + h) * p.Lq + q] = sum == 0.0f ? -__builtin_inff() : m + __log2f(sum);
+    }
 }
 
 // Sums along the diagonals of a 32 x 32 tile (lanes: queries, registers: keys), added to sums[key - query]; by one wave, in memory of its own.

@@ -60,13 +60,13 @@ template <typename F> hipError_t allow_lds(F kernel, std::atomic<uint32_t>& done
     return e;
 }
 // (kernels that share a type have a flag each: the address of one instance is a template argument)
-template <auto KERNEL, typename P> int launch(const char* name, dim3 grid, size_t lds, hipStream_t st, const P& p) {
+template <auto KERNEL, typename... P> int launch(const char* name, dim3 grid, size_t lds, hipStream_t st, const P&... p) {
     if (lds > 64 * 1024) {
         static std::atomic<uint32_t> done{0};
         const hipError_t e = allow_lds(KERNEL, done);
         if (e != hipSuccess) return hip_failed(name, e);
     }
-    KERNEL<<<grid, dim3(256), lds, st>>>(p);
+    KERNEL<<<grid, dim3(256), lds, st>>>(p...);
     LAUNCHED(name);
     return MFAR_OK;
 }
@@ -118,7 +118,28 @@ AttnParams attention_params(const mfar_attention* a) {
 int64_t drow_bytes(const mfar_attention* a) { return ((int64_t)a->B * a->H * a->Lq * 4 + 15) / 16 * 16; }
 size_t lut_bytes(const AttnParams& p) { return (size_t)(2 * (p.sat + AT_EDGE) + 1) * 4; }
 
-template <typename T, int DP> int attention_forward(const AttnParams& p, hipStream_t st) {
+// Up to 32 queries take the kernel that divides the keys over waves and blocks; a block gets at least 8 tiles of 32 keys, and there are no more
+// blocks than about four per CU.
+bool few_queries(const mfar_attention* a) { return a->Lq <= 32; }
+int key_splits(const mfar_attention* a) {
+    return (int)std::max<int64_t>(1, std::min(cdiv(1024, (int64_t)a->B * a->H), cdiv(a->Lk, 8 * 32)));
+}
+int64_t split_rows(const mfar_attention* a) { return (int64_t)a->B * a->Lq * a->H * key_splits(a); }
+int64_t split_bytes(const mfar_attention* a) { return few_queries(a) && key_splits(a) > 1 ? split_rows(a) * (a->D + 2) * 4 : 0; }
+
+template <typename T, int DP, bool KEEP> int attention_few(const AttnParams& p, const AttnSplit& sp, hipStream_t st) {
+    const size_t lds = 4ull * DP * 32 * 4 + 4 * 64 * 4 + lut_bytes(p);     // (the V tiles, 4 * 32 * DP elements, lie in its first part)
+    int rc = launch<mfar_attn_few_kernel<T, DP, KEEP>>("mfar_attn_few_kernel", dim3(sp.splits, p.H, p.B), lds, st, p, sp);
+    if (rc == MFAR_OK && sp.splits > 1)
+        rc = launch<mfar_attn_join_kernel<T, KEEP>>("mfar_attn_join_kernel", dim3(cdiv((int64_t)p.B * p.Lq * p.H, 4)), 0, st, p, sp);
+    return rc;
+}
+template <typename T, int DP> int attention_forward(const AttnParams& p, const AttnSplit& sp, hipStream_t st) {
+    if (sp.splits) {
+        if constexpr (sizeof(T) == 2)
+            if (p.out_lo) return attention_few<T, DP, true>(p, sp, st);
+        return attention_few<T, DP, false>(p, sp, st);
+    }
     const size_t lds = 2ull * AT_TILE * DP * sizeof(T) + lut_bytes(p);
     const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
     if constexpr (sizeof(T) == 2)
@@ -193,15 +214,19 @@ int64_t padded_k(int K) { return cdiv(K, 128) * 128; }
 extern "C" int64_t mfar_attention_workspace_bytes(const mfar_attention* a, int backward) {
     const int rc = check_attention(a, false);
     if (rc != MFAR_OK) return rc;
-    if (!backward || a->B == 0 || a->Lq == 0) return 0;
+    if (a->B == 0 || a->Lq == 0) return 0;
+    if (!backward) return split_bytes(a);
     return drow_bytes(a) + (a->dtable ? cdiv(a->Lq, AT_COLS) * a->B * a->H * a->n_buckets * 4 : 0);
 }
 extern "C" int mfar_attention_forward(int device, const mfar_attention* a, void* stream) {
     int rc = check_attention(a, false);
     if (rc != MFAR_OK || a->B == 0 || a->Lq == 0) return rc;
+    if (split_bytes(a) && (!a->workspace || a->workspace_bytes < split_bytes(a))) return bad("workspace too small");
     ON_DEVICE(device);
     const AttnParams p = attention_params(a);
-    return FOR_TYPE_AND_DIM(attention_forward, p, (hipStream_t)stream);
+    AttnSplit sp = {};
+    if (few_queries(a)) sp = {(float*)a->workspace, (float*)a->workspace + split_rows(a) * a->D, key_splits(a)};
+    return FOR_TYPE_AND_DIM(attention_forward, p, sp, (hipStream_t)stream);
 }
 extern "C" int mfar_attention_backward(int device, const mfar_attention* a, void* stream) {
     int rc = check_attention(a, true);
