@@ -192,13 +192,18 @@ int check_distill(const void* x, int dtype, int64_t ld, int64_t T, int64_t N, co
 }
 
 // ---- 8-bit linear -----------------------------------------------------------------------------------------------------------------------
-template <typename T> int quantize_rows(const void* x, int64_t ldx, int64_t M, int K, int8_t* q, int64_t ldq, float* scale, int pad, hipStream_t st) {
-    mfar_quantize_rows_kernel<T><<<cdiv(M, 4), 256, 0, st>>>((const T*)x, ldx, (int)M, K, (signed char*)q, ldq, scale, pad);
+template <typename T>
+int quantize_rows(const void* x, int64_t ldx, int64_t M, int K, int8_t* q, int64_t ldq, float* scale, int pad, const Int8Copy& cp, hipStream_t st) {
+    const int64_t blocks = cdiv(M, 4) + std::min<int64_t>(256, cdiv(cp.rows, 4));
+    mfar_quantize_rows_kernel<T><<<blocks, 256, 0, st>>>((const T*)x, ldx, (int)M, K, (signed char*)q, ldq, scale, pad, cp);
     LAUNCHED("mfar_quantize_rows_kernel");
     return MFAR_OK;
 }
-template <typename T> int int8_gemm(const Int8Params& p, hipStream_t st) {
-    return launch<mfar_int8_gemm_kernel<T>>("mfar_int8_gemm_kernel", dim3(cdiv(p.N, Q8_TILE), cdiv(p.M, Q8_TILE)), 0, st, p);
+// Tiles of 128 x 128 need about a block per CU to pay; fewer take 32 x 32 tiles, whose blocks divide k.
+bool small_product(int64_t M, int64_t N) { return cdiv(M, Q8_TILE) * cdiv(N, Q8_TILE) < 128; }
+template <typename T> int int8_product(const Int8Params& p, hipStream_t st) {
+    if (small_product(p.M, p.N)) return launch<mfar_int8_tile_kernel<T>>("mfar_int8_tile_kernel", dim3(cdiv(p.N, 32), cdiv(p.M, 32)), 0, st, p);
+    return launch<mfar_int8_gemm_kernel<T>>("mfar_int8_gemm_kernel", dim3(cdiv(p.N, Q8_TILE) * cdiv(p.M, Q8_TILE)), 4 * Q8_TILE_BYTES, st, p);
 }
 int check_rows(const void* x, int dtype, int64_t ldx, int64_t M, int K) {
     if (!type_size(dtype)) return bad("dtype must be F32, BF16 or F16");
@@ -207,7 +212,10 @@ int check_rows(const void* x, int dtype, int64_t ldx, int64_t M, int K) {
     if (M > 1 && ldx < 0) return bad("rows must not run backwards");
     return MFAR_OK;
 }
-int64_t padded_k(int K) { return cdiv(K, 128) * 128; }
+int64_t padded_k(int K) { return cdiv(K, Q8_STEP) * Q8_STEP; }
+bool copies_weights(int64_t M, int64_t N, int K) { return K % 16 && !small_product(M, N); }   // rows have to start on 16 bytes
+int64_t int8_scales_at(int64_t M, int K) { return M * padded_k(K); }
+int64_t int8_weights_at(int64_t M, int K) { return int8_scales_at(M, K) + cdiv(M * 4, 16) * 16; }
 
 }  // namespace
 
@@ -246,11 +254,11 @@ extern "C" int mfar_quantize_rows(int device, const void* x, int dtype, int64_t 
     if (!q || !scale) return bad("NULL output");
     if (ldq < K) return bad("ldq must be at least K");
     ON_DEVICE(device);
-    return FOR_TYPE(dtype, quantize_rows, x, ldx, M, K, q, ldq, scale, 0, (hipStream_t)stream);
+    return FOR_TYPE(dtype, quantize_rows, x, ldx, M, K, q, ldq, scale, 0, Int8Copy{}, (hipStream_t)stream);
 }
-extern "C" int64_t mfar_int8_linear_workspace_bytes(int64_t M, int K) {
-    if (M < 0 || K < 1) return bad("M must be >= 0, K >= 1");
-    return M * padded_k(K) + cdiv(M * 4, 16) * 16;
+extern "C" int64_t mfar_int8_linear_workspace_bytes(int64_t M, int K, int N) {
+    if (M < 0 || K < 1 || N < 0) return bad("M and N must be >= 0, K >= 1");
+    return int8_weights_at(M, K) + (copies_weights(M, N, K) ? (int64_t)N * padded_k(K) : 0);
 }
 extern "C" int mfar_int8_linear(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int N, const int8_t* wq, const float* w_scale,
                                 const float* bias, void* y, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -259,16 +267,24 @@ extern "C" int mfar_int8_linear(int device, const void* x, int dtype, int64_t ld
     if (N < 0 || N > (1 << 23)) return bad("N must be 0..2^23");
     if (M == 0 || N == 0) return MFAR_OK;
     if (!wq || !w_scale || !y) return bad("NULL tensor");
-    if (!workspace || !aligned16(workspace) || workspace_bytes < mfar_int8_linear_workspace_bytes(M, K)) return bad("workspace too small or not 16-byte aligned");
+    if (!aligned16(wq)) return bad("the weights must be 16-byte aligned");
+    if (!workspace || !aligned16(workspace) || workspace_bytes < mfar_int8_linear_workspace_bytes(M, K, N)) return bad("workspace too small or not 16-byte aligned");
     ON_DEVICE(device);
     const int64_t Kp = padded_k(K);
     int8_t* xq = (int8_t*)workspace;
-    float* xs = (float*)((char*)workspace + M * Kp);
+    float* xs = (float*)((char*)workspace + int8_scales_at(M, K));
     hipStream_t st = (hipStream_t)stream;
-    rc = FOR_TYPE(dtype, quantize_rows, x, ldx, M, K, xq, Kp, xs, 1, st);
+    Int8Copy cp = {};
+    const signed char* w = (const signed char*)wq;
+    int64_t ldw = K;
+    if (copies_weights(M, N, K)) {
+        cp = {w, (signed char*)workspace + int8_weights_at(M, K), (long long)Kp, N, K};
+        w = cp.to, ldw = Kp;
+    }
+    rc = FOR_TYPE(dtype, quantize_rows, x, ldx, M, K, xq, Kp, xs, 1, cp, st);
     if (rc != MFAR_OK) return rc;
-    const Int8Params p = {(const signed char*)xq, (const signed char*)wq, xs, w_scale, bias, y, (long long)Kp, (long long)K, (int)M, N, K, (int)Kp};
-    return FOR_TYPE(dtype, int8_gemm, p, st);
+    const Int8Params p = {(const signed char*)xq, w, xs, w_scale, bias, y, (long long)Kp, (long long)ldw, (int)M, N, K, (int)Kp};
+    return FOR_TYPE(dtype, int8_product, p, st);
 }
 
 extern "C" int64_t mfar_distill_workspace_bytes(int64_t T, int64_t N) {

@@ -56,10 +56,12 @@ def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: 
             raise ValueError(f"expected a float bias [{N}], got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.detach().float().contiguous()
     wq, w_scale = wq.contiguous(), w_scale.contiguous()
+    if wq.data_ptr() % 16:
+        wq = wq.clone()
     y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
     r = _rows(x)
     L = _native.lib()
-    n = L.mfar_int8_linear_workspace_bytes(r.shape[0], K)
+    n = L.mfar_int8_linear_workspace_bytes(r.shape[0], K, N)
     with torch.cuda.device(dev):
         work = torch.empty(n, dtype=torch.uint8, device=x.device)
         _native.check(L.mfar_int8_linear(dev, r.data_ptr(), _native.op_dtype(x), r.stride(0), r.shape[0], K, N, wq.data_ptr(), w_scale.data_ptr(),
