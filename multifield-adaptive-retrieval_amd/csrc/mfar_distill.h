@@ -100,13 +100,48 @@ template <typename T> __device__ void di_row_loss(const DistillParams& p, int ro
     }
 }
 
+// A piece [lo, hi) of a row, as wide loads see it: `step(i, v, n)` is called by one thread for each run of up to EACH elements, of which the first n
+// (EACH but at the row's ends) are real.  Rows may start anywhere; the runs start on 16 bytes.
+template <typename T> struct DiRun {
+    static constexpr int EACH = 16 / sizeof(T);
+    typedef T V __attribute__((ext_vector_type(EACH)));
+};
+// elements before the first 16-byte border at or behind `at`
+template <typename T> __device__ __forceinline__ int di_head(const T* at) { return (int)((16 - ((uintptr_t)at & 15)) & 15) / (int)sizeof(T); }
+
 template <typename T>
 __global__ __launch_bounds__(DI_BLOCK) void mfar_distill_forward_kernel(const DistillParams p) {
     const int row = blockIdx.x, lo = blockIdx.y * p.chunk, hi = min(p.N, lo + p.chunk);
     const T* x = (const T*)p.x + (long long)row * p.x_row;
     const float c = LOG2E / p.tau;
+    constexpr int E = DiRun<T>::EACH, U = 16 / E;                           // 16 elements a thread and turn
+    typedef typename DiRun<T>::V V;
+    const int first = min(hi, lo + di_head(x + lo)), runs = (hi - first) / E, last = first + runs * E;
+    const V* xv = (const V*)(x + first);
     float m = -__builtin_inff(), s = 0.0f;
-    for (int j = lo + (int)threadIdx.x; j < hi; j += DI_BLOCK) di_join(m, s, (float)x[j] * c, 1.0f);
+    for (int i = threadIdx.x; i < runs; i += U * DI_BLOCK) {
+        V v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = xv[min(i + u * DI_BLOCK, runs - 1)];
+        float t[16], top = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                t[u * E + e] = i + u * DI_BLOCK < runs ? (float)v[u][e] * c : -__builtin_inff();
+                top = fmaxf(top, t[u * E + e]);
+            }
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+        s *= exp2_fast(m - base);
+        m = top;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s += exp2_fast(t[e] - base);
+    }
+    // what lies before the first and behind the last whole run: at most 2 (E - 1) elements
+    {
+        const int k = threadIdx.x, j = k < first - lo ? lo + k : last + k - (first - lo);
+        if (j < hi && (j < first || j >= last)) di_join(m, s, (float)x[j] * c, 1.0f);
+    }
     di_join_block(m, s);
     if (p.splits > 1) {
         if (threadIdx.x == 0) {
@@ -152,7 +187,29 @@ __global__ __launch_bounds__(DI_BLOCK) void mfar_distill_backward_kernel(const D
     __syncthreads();
     for (int k = 0; k < p.K; ++k) mass += prob[k];
     mass = mass > 0.5f ? 1.0f : (mass == 0.0f ? 0.0f : mass);
-    for (int j = lo + (int)threadIdx.x; j < hi; j += DI_BLOCK) dx[j] = (T)(g * (mass == 0.0f ? 0.0f : mass * exp2_fast((float)x[j] * c - lse)));
+    const float scale = mass == 0.0f ? 0.0f : g * mass;
+    auto grad = [&](float v) { return (T)(mass == 0.0f ? 0.0f : scale * exp2_fast(v * c - lse)); };
+    constexpr int E = DiRun<T>::EACH;
+    typedef typename DiRun<T>::V V;
+    // runs start where dx has a 16-byte border; x is read wherever that falls
+    const int first = min(hi, lo + di_head(dx + lo)), runs = (hi - first) / E, last = first + runs * E;
+    for (int i = threadIdx.x; i < runs; i += 2 * DI_BLOCK) {
+        V v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) __builtin_memcpy(&v[u], x + first + min(i + u * DI_BLOCK, runs - 1) * E, sizeof(V));
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (i + u * DI_BLOCK < runs) {
+                V o;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = grad((float)v[u][e]);
+                *(V*)(dx + first + (i + u * DI_BLOCK) * E) = o;
+            }
+    }
+    {
+        const int k = threadIdx.x, j = k < first - lo ? lo + k : last + k - (first - lo);
+        if (j < hi && (j < first || j >= last)) dx[j] = grad((float)x[j]);
+    }
     __threadfence_block();
     __syncthreads();
     for (int k = threadIdx.x; k < p.K; k += DI_BLOCK) {

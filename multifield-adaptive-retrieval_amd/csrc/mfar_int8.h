@@ -122,6 +122,7 @@ struct Int8Params {
     const float *xs, *ws, *bias;
     void* y;
     long long ldx, ldw;
+    bool whole_rows;             // rows of y start on 16 bytes
     int M, N, K, Kp;             // Kp: K rounded up to Q8_STEP; xq rows hold zeros in [K, Kp)
 };
 
@@ -139,7 +140,7 @@ template <typename T> __device__ __forceinline__ void q8_store(const Int8Params&
         for (int j = 0; j < 4; ++j) {
             const int at = min(n + j, p.N - 1);
             const float v = (float)acc[4 * g + j] * xs * p.ws[at];
-            o[j] = (T)(p.bias ? v + p.bias[at] : v);
+            o[j] = (T)(v + (p.bias ? p.bias[at] : 0.0f));
         }
         if (n + 4 <= p.N) __builtin_memcpy(y + n, &o, sizeof o);
         else
@@ -194,76 +195,157 @@ __global__ __launch_bounds__(256) void mfar_int8_tile_kernel(const Int8Params p)
     q8_store<T>(p, acc, n0, m0 + (l & 31));
 }
 
-// ---- many tiles: 128 channels x 128 tokens per block, 4 waves of 64 x 64, k steps of 128 bytes ---------------------------------------------------
-// Both operands go straight from memory to LDS, two steps' buffers in turn, one barrier a step.  A wave's load instruction fills 8 rows of 128 bytes
-// in lane order; the swizzle (chunk c of row r at place c ^ (r / 2 % 8): 16 rows at one chunk meet 64 different banks) is applied on the
-// addresses the lanes load from.  Rows of both operands start on 16 bytes.
+// ---- many tiles ------------------------------------------------------------------------------------------------------------------------------------
+// A block computes TN channels x TM tokens with WN x WM waves of I x J tiles each, in k steps of 128 bytes (whole cache lines: steps of 64 bytes in a
+// deeper ring were 15 % slower).  Both operands go straight from memory to LDS, two steps' buffers in turn, one barrier a step.  A load
+// instruction of a wave fills 8 rows of 128 bytes in lane order; the swizzle (chunk c of row r at place c ^ (r / 2 % 8): 16 rows at one chunk meet
+// 64 different banks) is applied on the addresses the lanes load from.  Rows of both operands start on 16 bytes.
 __device__ __forceinline__ int q8_swz(int r) { return (r >> 1) & 7; }
-#define Q8_TILE 128
-#define Q8_TILE_BYTES (Q8_TILE * Q8_STEP)
-
 __device__ __forceinline__ void q8_to_lds(const signed char* base, u32 off, u32 lds) {
     asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
 
-template <typename T>
-__global__ __launch_bounds__(256, 2) void mfar_int8_gemm_kernel(const Int8Params p) {
-    extern __shared__ __align__(16) signed char q8_lds[];                  // [2][weights, tokens][128][128]
+template <int WN, int WM, int I, int J> struct Int8Shape {
+    static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES, TN = WN * I * 32, TM = WM * J * 32, BYTES = (TN + TM) * Q8_STEP;
+    static constexpr int LDS = 2 * BYTES + (2 * TN + TM) * 4;
+    static_assert(TN * Q8_STEP % (1024 * WAVES) == 0 && TM * Q8_STEP % (1024 * WAVES) == 0);
+    static_assert(WAVES * 32 * (64 * 4 + 16) <= 2 * BYTES && I % 2 == 0);
+};
+template <int I, int J> struct Int8Frags { i32x4 a[I], b[J]; };
+
+template <typename T, int WN, int WM, int I, int J>
+__global__ __launch_bounds__(64 * WN * WM, 2) void mfar_int8_gemm_kernel(const Int8Params p) {
+    typedef Int8Shape<WN, WM, I, J> S;
+    extern __shared__ __align__(16) signed char q8_lds[];                  // [2][weights TN, tokens TM][Q8_STEP]
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, half = l >> 5;
     // consecutive blocks go to the 8 XCDs in turn: an XCD takes a run of tiles, walked in groups of 4 token tiles, so that its L2 sees rows again
-    const int tn = (p.N + Q8_TILE - 1) / Q8_TILE, tm = (p.M + Q8_TILE - 1) / Q8_TILE, total = tn * tm, id = blockIdx.x;
-    const int per = total / 8, rest = total % 8, xcd = id % 8;
-    const int at = xcd * per + min(xcd, rest) + id / 8;
+    const int tn = (p.N + S::TN - 1) / S::TN, tm = (p.M + S::TM - 1) / S::TM, total = tn * tm, id = blockIdx.x;
+    const int xcd = id % 8, at = xcd * (total / 8) + min(xcd, total % 8) + id / 8;
     const int group = at / (4 * tn), rows = min(4, tm - group * 4), in = at - group * 4 * tn;
-    const int m0 = (group * 4 + in % rows) * Q8_TILE, n0 = in / rows * Q8_TILE;
+    const int m0 = (group * 4 + in % rows) * S::TM, n0 = in / rows * S::TN;
     const signed char* xb = p.xq + (long long)m0 * p.ldx;
     const signed char* wb = p.wq + (long long)n0 * p.ldw;
-    u32 xo[4], wo[4], wl[4];
+    constexpr int PW = S::TN * Q8_STEP / 1024 / S::WAVES, PX = S::TM * Q8_STEP / 1024 / S::WAVES;
+    u32 xo[PX], wo[PW], wl[PW];
     const int steps = p.Kp / Q8_STEP, cut = p.K - (steps - 1) * Q8_STEP;    // bytes of the last step that the weights have
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int r = (wave * 4 + t) * 8 + (l >> 3), c = (l & 7) ^ q8_swz(r);
-        const int wr = min(r, p.N - 1 - n0) * (int)p.ldw;
+    for (int t = 0; t < PW; ++t) {
+        const int r = (wave * PW + t) * 8 + (l >> 3), c = (l & 7) ^ q8_swz(r), row = min(r, p.N - 1 - n0) * (int)p.ldw;
+        wo[t] = (u32)(row + c * 16);
+        wl[t] = (u32)(row + (c * 16 < cut ? c * 16 : 0));                  // past the row's end: any bytes, x holds zeros there
+    }
+#pragma unroll
+    for (int t = 0; t < PX; ++t) {
+        const int r = (wave * PX + t) * 8 + (l >> 3), c = (l & 7) ^ q8_swz(r);
         xo[t] = (u32)(min(r, p.M - 1 - m0) * (int)p.ldx + c * 16);
-        wo[t] = (u32)(wr + c * 16);
-        wl[t] = (u32)(wr + (c * 16 < cut ? c * 16 : 0));                   // past the row's end: any bytes, x holds zeros there
     }
     const u32 lds = (u32)(uintptr_t)q8_lds;
     auto load = [&](int s) {
-        const u32 to = lds + (s & 1) * 2 * Q8_TILE_BYTES + wave * 4096;
+        const u32 to = lds + (s & 1) * S::BYTES + wave * PW * 1024, tx = lds + (s & 1) * S::BYTES + S::TN * Q8_STEP + wave * PX * 1024;
         const signed char *x = xb + s * Q8_STEP, *w = wb + s * Q8_STEP;
         const bool last = s == steps - 1;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) q8_to_lds(w, last ? wl[t] : wo[t], to + t * 1024);
+        for (int t = 0; t < PW; ++t) q8_to_lds(w, last ? wl[t] : wo[t], to + t * 1024);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) q8_to_lds(x, xo[t], to + Q8_TILE_BYTES + t * 1024);
+        for (int t = 0; t < PX; ++t) q8_to_lds(x, xo[t], tx + t * 1024);
     };
-    const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64;
-    i32x16 acc[2][2] = {};
+    // the tile's scales and bias, for the epilogue
+    float* channels = (float*)(q8_lds + 2 * S::BYTES);                // [2][TN] scales, bias
+    float* tokens = channels + 2 * S::TN;                                  // [TM] scales
+    for (int i = threadIdx.x; i < S::TN; i += S::THREADS) {
+        const int n = min(n0 + i, p.N - 1);
+        channels[i] = p.ws[n];
+        channels[S::TN + i] = p.bias ? p.bias[n] : 0.0f;
+    }
+    for (int i = threadIdx.x; i < S::TM; i += S::THREADS) tokens[i] = p.xs[min(m0 + i, p.M - 1)];
+
+    const int wn = wave % WN * I * 32, wm = wave / WN * J * 32;
+    i32x16 acc[I][J] = {};
+    // Fragments are read a quarter step ahead of their products: while the matrix units work on one quarter, the next (of this step, or the first of the
+    // next step, behind its wait and barrier) comes from LDS.
+    Int8Frags<I, J> f[2];
+    auto read = [&](Int8Frags<I, J>& to, int s, int u) {
+        const signed char* wt = q8_lds + (s & 1) * S::BYTES;
+        const signed char* xt = wt + S::TN * Q8_STEP;
+        const int c = 2 * u + half;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int r = wn + 32 * i + (l & 31);
+            to.a[i] = *(const i32x4*)(wt + r * Q8_STEP + ((c ^ q8_swz(r)) << 4));
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int r = wm + 32 * j + (l & 31);
+            to.b[j] = *(const i32x4*)(xt + r * Q8_STEP + ((c ^ q8_swz(r)) << 4));
+        }
+    };
+    auto multiply = [&](const Int8Frags<I, J>& g) {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(g.a[i], g.b[j], acc[i][j], 0, 0, 0);
+    };
+    // a step is there once every wave has waited for its own loads; by then every wave also holds its last fragments of the step before
+    auto arrive = [&]() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
     load(0);
+    arrive();
+    if (steps > 1) load(1);
+    read(f[0], 0, 0);
     for (int s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                    // this wave's loads of step s
-        __syncthreads();                                                   // everyone's; and step s - 1 has been read
-        if (s + 1 < steps) load(s + 1);
-        const signed char* wt = q8_lds + (s & 1) * 2 * Q8_TILE_BYTES;
-        const signed char* xt = wt + Q8_TILE_BYTES;
+        read(f[1], s, 1);
+        multiply(f[0]);
+        read(f[0], s, 2);
+        multiply(f[1]);
+        read(f[1], s, 3);
+        multiply(f[0]);
+        if (s + 1 < steps) {
+            arrive();
+            if (s + 2 < steps) load(s + 2);
+            read(f[0], s + 1, 0);
+        }
+        multiply(f[1]);
+    }
+    if (!p.whole_rows) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            i32x4 a[2], b[2];
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int rn = wn + 32 * i + (l & 31), rm = wm + 32 * i + (l & 31), c = 2 * u + half;
-                a[i] = *(const i32x4*)(wt + rn * 128 + ((c ^ q8_swz(rn)) << 4));
-                b[i] = *(const i32x4*)(xt + rm * 128 + ((c ^ q8_swz(rm)) << 4));
-            }
+            for (int i = 0; i < I; ++i) q8_store<T>(p, acc[i][j], n0 + wn + 32 * i, m0 + wm + 32 * j + (l & 31));
+        return;
+    }
+    // Scaled results through LDS of the wave's own, 32 tokens x 64 channels at a time, so that a token's channels leave in runs of 16 bytes a lane
+    // (8 bytes a lane of 32 different tokens straight from the registers: twice the time at 32768 x 768 x 1536)
+    constexpr int PITCH = 64 * sizeof(T) + 16, LANES = 64 * sizeof(T) / 16, EACH = 16 / sizeof(T);
+    __syncthreads();
+    signed char* mine = q8_lds + wave * 32 * PITCH;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const float xs = tokens[wm + 32 * j + (l & 31)];
+#pragma unroll
+        for (int i0 = 0; i0 < I; i0 += 2) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+                for (int g = 0; g < 4; ++g) {
+                    const int n = 32 * i + 8 * g + 4 * half;
+                    const f32x4 ws = *(const f32x4*)(channels + wn + 32 * i0 + n), bias = *(const f32x4*)(channels + S::TN + wn + 32 * i0 + n);
+                    V4<T> o;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = (T)((float)acc[i0 + i][j][4 * g + e] * xs * ws[e] + bias[e]);
+                    *(V4<T>*)(mine + (l & 31) * PITCH + n * sizeof(T)) = o;
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += 64 / LANES) {
+                const int r = r0 + l / LANES, c = l % LANES, m = m0 + wm + 32 * j + r, n = n0 + wn + 32 * i0 + c * EACH;
+                const i32x4 x = *(const i32x4*)(mine + r * PITCH + c * 16);
+                if (m < p.M && n < p.N) *(i32x4*)((T*)p.y + (long long)m * p.N + n) = x;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) q8_store<T>(p, acc[i][j], n0 + wn + 32 * i, m0 + wm + 32 * j + (l & 31));
 }

@@ -200,10 +200,25 @@ int quantize_rows(const void* x, int64_t ldx, int64_t M, int K, int8_t* q, int64
     return MFAR_OK;
 }
 // Tiles of 128 x 128 need about a block per CU to pay; fewer take 32 x 32 tiles, whose blocks divide k.
-bool small_product(int64_t M, int64_t N) { return cdiv(M, Q8_TILE) * cdiv(N, Q8_TILE) < 128; }
+bool small_product(int64_t M, int64_t N) { return cdiv(M, 128) * cdiv(N, 128) < 128; }
+template <typename T, int WN, int WM, int I, int J> int int8_gemm(const Int8Params& p, hipStream_t st) {
+    typedef Int8Shape<WN, WM, I, J> S;
+    static std::atomic<uint32_t> done{0};
+    auto kernel = mfar_int8_gemm_kernel<T, WN, WM, I, J>;
+    if (S::LDS > 64 * 1024) {
+        const hipError_t e = allow_lds(kernel, done);
+        if (e != hipSuccess) return hip_failed("mfar_int8_gemm_kernel", e);
+    }
+    kernel<<<cdiv(p.N, S::TN) * cdiv(p.M, S::TM), S::THREADS, S::LDS, st>>>(p);
+    LAUNCHED("mfar_int8_gemm_kernel");
+    return MFAR_OK;
+}
 template <typename T> int int8_product(const Int8Params& p, hipStream_t st) {
     if (small_product(p.M, p.N)) return launch<mfar_int8_tile_kernel<T>>("mfar_int8_tile_kernel", dim3(cdiv(p.N, 32), cdiv(p.M, 32)), 0, st, p);
-    return launch<mfar_int8_gemm_kernel<T>>("mfar_int8_gemm_kernel", dim3(cdiv(p.N, Q8_TILE) * cdiv(p.M, Q8_TILE)), 4 * Q8_TILE_BYTES, st, p);
+    // Tiles of 256 x 256 move half the bytes per product but take a CU each: with a tile for every CU they win (16384 x 4096 x 4096: 287 us against 335;
+    // 32768 x 768 x 1536: 54 against 62), with half as many they lose (8192 x 4096 x 1024: 84 us against 70, quantising included).
+    if (cdiv(p.M, 256) * cdiv(p.N, 256) >= 256) return int8_gemm<T, 2, 4, 4, 2>(p, st);
+    return int8_gemm<T, 2, 2, 2, 2>(p, st);
 }
 int check_rows(const void* x, int dtype, int64_t ldx, int64_t M, int K) {
     if (!type_size(dtype)) return bad("dtype must be F32, BF16 or F16");
@@ -283,7 +298,8 @@ extern "C" int mfar_int8_linear(int device, const void* x, int dtype, int64_t ld
     }
     rc = FOR_TYPE(dtype, quantize_rows, x, ldx, M, K, xq, Kp, xs, 1, cp, st);
     if (rc != MFAR_OK) return rc;
-    const Int8Params p = {(const signed char*)xq, w, xs, w_scale, bias, y, (long long)Kp, (long long)ldw, (int)M, N, K, (int)Kp};
+    const Int8Params p = {(const signed char*)xq, w, xs, w_scale, bias, y, (long long)Kp, (long long)ldw,
+                          (int64_t)N * type_size(dtype) % 16 == 0 && aligned16(y), (int)M, N, K, (int)Kp};
     return FOR_TYPE(dtype, int8_product, p, st);
 }
 

@@ -291,7 +291,7 @@ def _int8_check(x, wq, ws, b, got):
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 768, 768), (12, 768, 769), (33, 64, 96), (129, 1001, 519), (300, 130, 257), (1000, 1536, 768), (70, 4096, 33),
-                                   (513, 17, 1030), (3000, 200, 1500), (2049, 1000, 1025), (1700, 136, 1700)])
+                                   (513, 17, 1030), (3000, 200, 1500), (2049, 1000, 1025), (1700, 136, 1700), (4100, 144, 4200), (4000, 300, 4097)])
 def test_int8_linear(dtype, M, K, N):
     from mfar.modeling.quantized import int8_linear
     print(f"int8 {dtype} {M} {K} {N}", flush=True)
