@@ -553,14 +553,14 @@ int mfar_int8_linear(int device, const void* x, int dtype, int64_t ldx, int64_t 
 /*
  * Distillation from a teacher's top scores: p = softmax(scores / tau) over a row's ids >= 0, q = softmax(student / tau) over its N columns;
  * loss[t] = tau^2 KL(p || q).  A row without ids: loss and gradient 0.  An id >= N: the row's loss and gradient are NaN.  An id may repeat.
- * student [T, N] rows ld elements apart; ids [T, K] int64, scores [T, K] fp32, K <= 1024; prob [T, K] and lse [T] are kept for the backward
+ * student [T, N] rows ld elements apart; ids [T, K] int64, scores [T, K] fp32, K <= 1024; prob [T, K] and stat [T, 2] are kept for the backward
  * pass; dstudent [T, N] contiguous, of the student's type; dloss [T].
  */
 int64_t mfar_distill_workspace_bytes(int64_t T, int64_t N);
 int mfar_distill_forward(int device, const void* student, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, const float* scores, int K,
-                         float tau, float* loss, float* prob, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+                         float tau, float* loss, float* prob, float* stat, void* workspace, int64_t workspace_bytes, void* stream);
 int mfar_distill_backward(int device, const void* student, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, int K, float tau,
-                          const float* prob, const float* lse, const float* dloss, void* dstudent, void* stream);
+                          const float* prob, const float* stat, const float* dloss, void* dstudent, void* stream);
 
 #ifdef __cplusplus
 }

@@ -309,26 +309,26 @@ extern "C" int64_t mfar_distill_workspace_bytes(int64_t T, int64_t N) {
     return splits > 1 ? T * splits * 8 : 0;
 }
 extern "C" int mfar_distill_forward(int device, const void* student, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, const float* scores,
-                                    int K, float tau, float* loss, float* prob, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+                                    int K, float tau, float* loss, float* prob, float* stat, void* workspace, int64_t workspace_bytes, void* stream) {
     const int rc = check_distill(student, dtype, ld, T, N, ids, K, tau);
     if (rc != MFAR_OK || T == 0) return rc;
-    if (!scores || !loss || !prob || !lse) return bad("NULL tensor");
+    if (!scores || !loss || !prob || !stat) return bad("NULL tensor");
     const int64_t need = mfar_distill_workspace_bytes(T, N);
     if (need && (!workspace || workspace_bytes < need)) return bad("workspace too small");
     ON_DEVICE(device);
     DistillParams p = {};
-    p.x = student, p.x_row = ld, p.ids = (const long long*)ids, p.scores = scores, p.loss = loss, p.prob = prob, p.lse = lse, p.part = (float*)workspace;
+    p.x = student, p.x_row = ld, p.ids = (const long long*)ids, p.scores = scores, p.loss = loss, p.prob = prob, p.stat = stat, p.part = (float*)workspace;
     p.T = (int)T, p.N = (int)N, p.K = K, p.chunk = distill_chunk(T, N), p.splits = (int)cdiv(N, p.chunk), p.tau = tau;
     return FOR_TYPE(dtype, distill_forward, p, (hipStream_t)stream);
 }
 extern "C" int mfar_distill_backward(int device, const void* student, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, int K, float tau,
-                                     const float* prob, const float* lse, const float* dloss, void* dstudent, void* stream) {
+                                     const float* prob, const float* stat, const float* dloss, void* dstudent, void* stream) {
     const int rc = check_distill(student, dtype, ld, T, N, ids, K, tau);
     if (rc != MFAR_OK || T == 0) return rc;
-    if (!prob || !lse || !dloss || !dstudent) return bad("NULL tensor");
+    if (!prob || !stat || !dloss || !dstudent) return bad("NULL tensor");
     ON_DEVICE(device);
     DistillParams p = {};
-    p.x = student, p.x_row = ld, p.ids = (const long long*)ids, p.g = dloss, p.prob = (float*)prob, p.lse = (float*)lse, p.dx = dstudent;
+    p.x = student, p.x_row = ld, p.ids = (const long long*)ids, p.g = dloss, p.prob = (float*)prob, p.stat = (float*)stat, p.dx = dstudent;
     p.T = (int)T, p.N = (int)N, p.K = K, p.chunk = distill_chunk(T, N), p.splits = (int)cdiv(N, p.chunk), p.tau = tau;
     return FOR_TYPE(dtype, distill_backward, p, (hipStream_t)stream);
 }

@@ -90,27 +90,28 @@ class _TopKDistillation(torch.autograd.Function):
         T, N = student.shape
         K = ids.shape[1]
         x = student if student.stride(1) == 1 or N == 1 else student.contiguous()
-        loss, lse = (torch.empty(T, dtype=torch.float32, device=x.device) for _ in range(2))
+        loss = torch.empty(T, dtype=torch.float32, device=x.device)
         prob = torch.empty(T, K, dtype=torch.float32, device=x.device)
+        stat = torch.empty(T, 2, dtype=torch.float32, device=x.device)
         L = _native.lib()
         n = L.mfar_distill_workspace_bytes(T, N)
         work = torch.empty(max(0, n), dtype=torch.uint8, device=x.device)
         _native.check(L.mfar_distill_forward(dev, x.data_ptr(), _native.op_dtype(x), x.stride(0), T, N, ids.data_ptr(), scores.data_ptr(), K, tau,
-                                             loss.data_ptr(), prob.data_ptr(), lse.data_ptr(), work.data_ptr(), n, _native.op_stream(dev)))
-        ctx.save_for_backward(x, ids, prob, lse)
+                                             loss.data_ptr(), prob.data_ptr(), stat.data_ptr(), work.data_ptr(), n, _native.op_stream(dev)))
+        ctx.save_for_backward(x, ids, prob, stat)
         ctx.tau = tau
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, ids, prob, lse = ctx.saved_tensors
+        x, ids, prob, stat = ctx.saved_tensors
         dev = x.device.index
         T, N = x.shape
         dx = torch.empty(T, N, dtype=x.dtype, device=x.device)
         dloss = dloss.float().contiguous()
         _native.check(_native.lib().mfar_distill_backward(dev, x.data_ptr(), _native.op_dtype(x), x.stride(0), T, N, ids.data_ptr(), ids.shape[1], ctx.tau,
-                                                          prob.data_ptr(), lse.data_ptr(), dloss.data_ptr(), dx.data_ptr(), _native.op_stream(dev)))
+                                                          prob.data_ptr(), stat.data_ptr(), dloss.data_ptr(), dx.data_ptr(), _native.op_stream(dev)))
         return dx, None, None, None
 
 
