@@ -169,10 +169,16 @@ def check(rc: int):
         raise MfarError(rc, lib().mfar_last_error().decode("utf-8", "replace"))
 
 
+_OP_DTYPES = None
+
+
 def op_dtype(t) -> int:
     """Type code of a tensor handed to an encoder / training operator."""
-    import torch
-    code = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}.get(t.dtype)
+    global _OP_DTYPES
+    if _OP_DTYPES is None:
+        import torch
+        _OP_DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+    code = _OP_DTYPES.get(t.dtype)
     if code is None:
         raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}")
     return code
@@ -186,15 +192,18 @@ def op_device(*tensors) -> int:
             continue
         if not t.is_cuda:
             raise ValueError(f"expected a tensor on the GPU, got one on {t.device}")
-        if dev is not None and t.device.index != dev:
-            raise ValueError(f"tensors live on cuda:{dev} and {t.device}")
-        dev = t.device.index
+        d = t.get_device()
+        if dev is None:
+            dev = d
+        elif d != dev:
+            raise ValueError(f"tensors live on cuda:{dev} and cuda:{d}")
     return dev
 
 
 def op_stream(device: int) -> int:
+    """The caller's current stream on `device`."""
     import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def device_count() -> int:

@@ -46,45 +46,45 @@ def relative_buckets(distance: torch.Tensor, num_buckets: int, causal: bool, max
     return b if causal else b + side * (distance > 0).to(b.dtype)
 
 
-def _strided(x: torch.Tensor) -> torch.Tensor:
-    """x as the kernels can read it: last dim contiguous, rows and base on 16-byte boundaries; copied where it is not."""
+@functools.lru_cache(maxsize=64)
+def _borders(num_buckets: int, causal: bool, max_distance: int):
+    b = bucket_borders(num_buckets, causal, max_distance)
+    return ctypes.cast(b, ctypes.POINTER(ctypes.c_int32)), len(b)      # (the pointer keeps the array alive)
+
+
+def _layout(x: torch.Tensor):
+    """(x as the kernels can read it, its strides over batch, rows and heads): last dim contiguous, rows and base on 16-byte boundaries, row
+    strides of at most 2^22 elements; copied where it is not."""
+    b, l, h, d = x.stride()
     es = x.element_size()
-    ok = x.stride(3) == 1 or x.size(3) == 1
-    ok = ok and x.data_ptr() % 16 == 0 and all(x.stride(i) * es % 16 == 0 or x.size(i) == 1 for i in range(3))
-    ok = ok and (x.size(1) == 1 or x.stride(1) <= 2 ** 22)
-    return x if ok else x.contiguous()
-
-
-def _set(a, name, x):
-    setattr(a, name, x.data_ptr())
-    p = "do" if name == "dout" else name
-    for i, d in enumerate("blh"):
-        setattr(a, f"{p}_{d}", x.stride(i) if x.size(i) > 1 else 0)
+    if d == 1 and l <= 4194304 and not ((b | l | h) * es | x.data_ptr()) & 15:
+        return x, b, (l if x.size(1) > 1 else 0), h
+    n = x.size()
+    b, l, h = (0 if n[i] == 1 else s for i, s in enumerate((b, l, h)))    # (a dim of one element may have any stride)
+    if (d != 1 and n[3] != 1) or l > 4194304 or ((b | l | h) * es | x.data_ptr()) & 15:
+        x = x.contiguous()
+        b, l, h = n[1] * n[2] * n[3], n[2] * n[3], n[3]
+        if x.data_ptr() & 15:
+            x = x.clone()
+    return x, b, l, h
 
 
 def _call(q, k, v, table, key_mask, q_start, causal, borders, scale):
-    """The C struct of one call's inputs (the tensors must outlive it)."""
-    a = _native.Attention()
-    a.dtype = _native.op_dtype(q)
-    a.B, a.Lq, a.H, a.D = q.shape
-    a.Lk = k.shape[1]
-    a.causal, a.n_buckets, a.n_borders, a.scale = int(causal), table.shape[0], len(borders), scale
-    a.borders = ctypes.cast(borders, ctypes.POINTER(ctypes.c_int32))
-    a.table = table.data_ptr()
-    _set(a, "q", q)
-    _set(a, "k", k)
-    _set(a, "v", v)
-    if key_mask is not None:
-        a.key_mask, a.mask_b = key_mask.data_ptr(), key_mask.stride(0) if key_mask.size(0) > 1 else 0
-    if torch.is_tensor(q_start):
-        a.q_start_each = q_start.data_ptr()
-    else:
-        a.q_start = q_start
-    return a
+    """(the C struct of one call's inputs, the tensors that must outlive it)."""
+    q, q_b, q_l, q_h = _layout(q)
+    k, k_b, k_l, k_h = _layout(k)
+    v, v_b, v_l, v_h = _layout(v)
+    B, Lq, H, D = q.shape
+    each = torch.is_tensor(q_start)
+    a = _native.Attention(_native.op_dtype(q), B, Lq, k.shape[1], H, D, causal, table.shape[0], borders[1], scale, borders[0], table.data_ptr(),
+                          q.data_ptr(), k.data_ptr(), v.data_ptr(), q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h,
+                          None if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None or B == 1 else key_mask.stride(0),
+                          q_start.data_ptr() if each else None, 0 if each else q_start)
+    return a, (q, k, v)
 
 
 def _workspace(a, backward, device):
-    n = _native.lib().mfar_attention_workspace_bytes(ctypes.byref(a), int(backward))
+    n = _native.lib().mfar_attention_workspace_bytes(a, backward)
     if n < 0:
         _native.check(int(n))
     if n == 0:
@@ -95,8 +95,7 @@ def _workspace(a, backward, device):
 
 
 def _forward(q, k, v, table, key_mask, q_start, causal, borders, scale, keep):
-    q, k, v = _strided(q), _strided(k), _strided(v)
-    a = _call(q, k, v, table, key_mask, q_start, causal, borders, scale)
+    a, (q, k, v) = _call(q, k, v, table, key_mask, q_start, causal, borders, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lo = lse = None
     a.out = out.data_ptr()
@@ -107,7 +106,8 @@ def _forward(q, k, v, table, key_mask, q_start, causal, borders, scale, keep):
             lo = torch.empty_like(out)
             a.out_lo = lo.data_ptr()
     work = _workspace(a, False, q.device)      # noqa: F841 -- alive until the call is enqueued
-    _native.check(_native.lib().mfar_attention_forward(q.device.index, ctypes.byref(a), _native.op_stream(q.device.index)))
+    dev = q.get_device()
+    _native.check(_native.lib().mfar_attention_forward(dev, a, _native.op_stream(dev)))
     return out, lo, lse, (q, k, v)
 
 
@@ -125,22 +125,22 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, table, key_mask, start, out, lo, lse = ctx.saved_tensors
         q_start, causal, borders, scale = ctx.rest
-        dout = _strided(dout)
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
         if q.numel() == 0 or k.numel() == 0:
             return dq.zero_(), dk.zero_(), dv.zero_(), torch.zeros_like(table), None, None, None, None, None
-        a = _call(q, k, v, table, key_mask, q_start if start is None else start, causal, borders, scale)
-        a.out, a.lse = out.data_ptr(), lse.data_ptr()
+        a, keep = _call(q, k, v, table, key_mask, q_start if start is None else start, causal, borders, scale)      # noqa: F841
+        dout, a.do_b, a.do_l, a.do_h = _layout(dout)
+        a.out, a.lse, a.dout = out.data_ptr(), lse.data_ptr(), dout.data_ptr()
         if lo is not None:
             a.out_lo = lo.data_ptr()
-        _set(a, "dout", dout)
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         dtable = None
         if ctx.needs_input_grad[3]:
             dtable = torch.empty_like(table)
             a.dtable = dtable.data_ptr()
         work = _workspace(a, True, q.device)      # noqa: F841
-        _native.check(_native.lib().mfar_attention_backward(q.device.index, ctypes.byref(a), _native.op_stream(q.device.index)))
+        dev = q.get_device()
+        _native.check(_native.lib().mfar_attention_backward(dev, a, _native.op_stream(dev)))
         return dq, dk, dv, dtable, None, None, None, None, None
 
 
@@ -179,14 +179,14 @@ def relative_bias_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, t
         q_start = q_start.clamp(-2 ** 30, 2 ** 30).to(torch.int32) if q_start.dtype == torch.int64 else q_start.contiguous()
     elif not -2 ** 30 <= q_start <= 2 ** 30:
         raise ValueError(f"q_start {q_start} is out of range")
-    borders = bucket_borders(table.shape[0], bool(causal), int(max_distance))
-    table = table.float().contiguous()
+    borders = _borders(table.shape[0], bool(causal), int(max_distance))
+    if table.dtype != torch.float32 or not table.is_contiguous():
+        table = table.float().contiguous()
     pad = -D % 8
     if pad:
         q, k, v = (torch.nn.functional.pad(x, (0, pad)) for x in (q, k, v))
-    with torch.cuda.device(dev):
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
-            out = _Attention.apply(q, k, v, table, key_mask, q_start, bool(causal), borders, float(scale))
-        else:
-            out = _forward(q, k, v, table, key_mask, q_start, bool(causal), borders, float(scale), False)[0]
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
+        out = _Attention.apply(q, k, v, table, key_mask, q_start, bool(causal), borders, float(scale))
+    else:
+        out = _forward(q, k, v, table, key_mask, q_start, bool(causal), borders, float(scale), False)[0]
     return out[..., :D] if pad else out

@@ -86,32 +86,32 @@ class HybridContrastiveLoss(torch.nn.Module):
 class _TopKDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, student, ids, scores, tau):
-        dev = student.device.index
+        dev = student.get_device()
         T, N = student.shape
         K = ids.shape[1]
         x = student if student.stride(1) == 1 or N == 1 else student.contiguous()
-        loss = torch.empty(T, dtype=torch.float32, device=x.device)
-        prob = torch.empty(T, K, dtype=torch.float32, device=x.device)
-        stat = torch.empty(T, 2, dtype=torch.float32, device=x.device)
         L = _native.lib()
         n = L.mfar_distill_workspace_bytes(T, N)
-        work = torch.empty(max(0, n), dtype=torch.uint8, device=x.device)
+        loss = torch.empty(T, dtype=torch.float32, device=x.device)
+        kept = torch.empty(T * (K + 2) + max(0, n) // 4, dtype=torch.float32, device=x.device)     # statistics [T, 2], probabilities [T, K], workspace
+        at = kept.data_ptr()
         _native.check(L.mfar_distill_forward(dev, x.data_ptr(), _native.op_dtype(x), x.stride(0), T, N, ids.data_ptr(), scores.data_ptr(), K, tau,
-                                             loss.data_ptr(), prob.data_ptr(), stat.data_ptr(), work.data_ptr(), n, _native.op_stream(dev)))
-        ctx.save_for_backward(x, ids, prob, stat)
+                                             loss.data_ptr(), at + 8 * T, at, at + 4 * T * (K + 2), n, _native.op_stream(dev)))
+        ctx.save_for_backward(x, ids, kept)
         ctx.tau = tau
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, ids, prob, stat = ctx.saved_tensors
-        dev = x.device.index
+        x, ids, kept = ctx.saved_tensors
+        dev = x.get_device()
         T, N = x.shape
         dx = torch.empty(T, N, dtype=x.dtype, device=x.device)
         dloss = dloss.float().contiguous()
+        at = kept.data_ptr()
         _native.check(_native.lib().mfar_distill_backward(dev, x.data_ptr(), _native.op_dtype(x), x.stride(0), T, N, ids.data_ptr(), ids.shape[1], ctx.tau,
-                                                          prob.data_ptr(), stat.data_ptr(), dloss.data_ptr(), dx.data_ptr(), _native.op_stream(dev)))
+                                                          at + 8 * T, at, dloss.data_ptr(), dx.data_ptr(), _native.op_stream(dev)))
         return dx, None, None, None
 
 
@@ -123,7 +123,7 @@ def topk_distillation(student: torch.Tensor, teacher_ids: torch.Tensor, teacher_
     student [T, N] float32 / float16 / bfloat16 on the GPU; teacher_ids [T, K] int64 or int32 columns, K <= 1024, negative: no entry (short
     lists); teacher_scores [T, K], used in fp32, no gradient.  A row without entries has loss 0 and gradient 0; an id past the last column
     makes its row NaN; a repeated id adds up."""
-    dev = _native.op_device(student, teacher_ids, teacher_scores)
+    _native.op_device(student, teacher_ids, teacher_scores)
     if student.dim() != 2 or student.shape[1] < 1 or student.shape[1] > 2 ** 30:
         raise ValueError(f"expected student scores [T, N], 1 <= N <= 2^30, got {tuple(student.shape)}")
     if teacher_ids.dtype not in (torch.int64, torch.int32) or teacher_ids.dim() != 2 or teacher_ids.shape[0] != student.shape[0]:
@@ -135,8 +135,7 @@ def topk_distillation(student: torch.Tensor, teacher_ids: torch.Tensor, teacher_
     if not 0.0 < temperature < float("inf"):
         raise ValueError(f"the temperature must be positive and finite, got {temperature}")
     _native.op_dtype(student)
-    with torch.cuda.device(dev):
-        return _TopKDistillation.apply(student, teacher_ids.to(torch.int64).contiguous(), teacher_scores.detach().float().contiguous(), float(temperature))
+    return _TopKDistillation.apply(student, teacher_ids.to(torch.int64).contiguous(), teacher_scores.detach().float().contiguous(), float(temperature))
 
 
 class TopKDistillationLoss(torch.nn.Module):

@@ -14,7 +14,7 @@ MAX_K = 131072
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """[..., K] as a 2-D view of rows with contiguous elements."""
-    r = x.reshape(-1, x.shape[-1])
+    r = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     return r if r.stride(1) == 1 or r.size(1) == 1 else r.contiguous()
 
 
@@ -62,8 +62,7 @@ def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: 
     r = _rows(x)
     L = _native.lib()
     n = L.mfar_int8_linear_workspace_bytes(r.shape[0], K, N)
-    with torch.cuda.device(dev):
-        work = torch.empty(n, dtype=torch.uint8, device=x.device)
-        _native.check(L.mfar_int8_linear(dev, r.data_ptr(), _native.op_dtype(x), r.stride(0), r.shape[0], K, N, wq.data_ptr(), w_scale.data_ptr(),
-                                         bias.data_ptr() if bias is not None else None, y.data_ptr(), work.data_ptr(), n, _native.op_stream(dev)))
+    work = torch.empty(n, dtype=torch.uint8, device=x.device)
+    _native.check(L.mfar_int8_linear(dev, r.data_ptr(), _native.op_dtype(x), r.stride(0), r.shape[0], K, N, wq.data_ptr(), w_scale.data_ptr(),
+                                     None if bias is None else bias.data_ptr(), y.data_ptr(), work.data_ptr(), n, _native.op_stream(dev)))
     return y
