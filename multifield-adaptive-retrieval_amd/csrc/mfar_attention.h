@@ -67,45 +67,56 @@ template <int DP> __device__ __forceinline__ int at_swz(int r) {
 }
 template <typename T, int DP> __device__ __forceinline__ T* at_at(T* tile, int r, int c) { return tile + r * DP + ((c ^ at_swz<DP>(r)) << 3); }
 
-// Tiles of AT_TILE rows of one (batch, head) on their way to LDS: fetch() loads one into registers (ahead of the step that needs it, so that the
-// loads run under the previous step's products), put() writes it.  Rows >= n are not read (the last row stands in); rows whose bit of `bits` is 0 and
-// dims >= D become zeros: a masked row may hold anything, also NaN, and must not reach a product.  Row strides fit 22 bits, so a lane's place in a
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
+// Steps of tiles held in LDS: two, so that one loads while the other is multiplied; one where two would leave a CU a single block.
+constexpr int at_stages(int size, int dp) { return size * dp >= 512 ? 1 : 2; }
+
+// Tiles of AT_TILE rows of one (batch, head) straight from memory to LDS: a wave's load instruction fills 1 KB in lane order, the swizzle of at_at is
+// applied on the addresses the lanes load from.  Rows >= n are not read (the last row stands in), nor are dims >= D (the row's first chunk stands in:
+// the other operand of every product holds zeros there, and results of those dims are dropped).  Row strides fit 22 bits, so a lane's place in a
 // tile is a 32-bit offset from a scalar address.
-template <typename T, int DP> struct AtTileIn {
-    static constexpr int CH = DP / 8, N = DP / 32;
+template <typename T, int DP> struct AtStream {
+    static constexpr int ROW = DP * sizeof(T), N = AT_TILE * ROW / 1024 / 4, PIECES = ROW / 16, EACH = sizeof(T) / 2;   // EACH: 16-byte pieces a chunk
     const T* base;
     long long stride;
-    int n, off[N];
-    bool in;                     // the lane's dims exist
-    V8<T> x[N];
-    __device__ __forceinline__ AtTileIn(const T* base_, long long stride_, int n_, int D) : base(base_), stride(stride_), n(n_) {
-        const int c = (int)threadIdx.x % CH;
-        in = c * 8 < D;
+    int n;
+    u32 off[N];
+    __device__ __forceinline__ AtStream(const T* base_, long long stride_, int n_, int D) : base(base_), stride(stride_), n(n_) {
+        const int piece = (threadIdx.x & 63) % PIECES;
 #pragma unroll
-        for (int t = 0; t < N; ++t) off[t] = row(t) * (int)stride + (in ? c * 8 : 0);
+        for (int t = 0; t < N; ++t) {
+            const int c = (piece / EACH) ^ at_swz<DP>(row(t));
+            off[t] = (u32)(row(t) * (int)stride + (c * 8 < D ? c * 8 : 0)) * (u32)sizeof(T) + (piece % EACH) * 16;
+        }
     }
-    static __device__ __forceinline__ int row(int t) { return (t * AT_BLOCK + (int)threadIdx.x) / CH; }
-    __device__ __forceinline__ void fetch(int r0) {
-        const T* at = base + (long long)r0 * stride;
+    static __device__ __forceinline__ int row(int t) { return (wave_index() * N + t) * (64 / PIECES) + (int)(threadIdx.x & 63) / PIECES; }
+    __device__ __forceinline__ void load(int r0, T* tile) const {
+        const u64 address = (u64)(uintptr_t)(base + (long long)r0 * stride);
+        const u64 at = ((u64)(u32)__builtin_amdgcn_readfirstlane((int)(address >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)address);
         const int over = r0 - (n - 1);
 #pragma unroll
-        for (int t = 0; t < N; ++t) x[t] = *(const V8<T>*)(at + (off[t] - __mul24(max(0, over + row(t)), (int)stride)));
-    }
-    __device__ __forceinline__ void put(T* tile, u64 bits, bool whole) const {
-        const int c = (int)threadIdx.x % CH;
-        if (bits == ~0ull && whole) {
-#pragma unroll
-            for (int t = 0; t < N; ++t) *(V8<T>*)at_at<T, DP>(tile, row(t), c) = x[t];
-        } else {
-#pragma unroll
-            for (int t = 0; t < N; ++t) *(V8<T>*)at_at<T, DP>(tile, row(t), c) = in && ((bits >> row(t)) & 1) ? x[t] : V8<T>{};
+        for (int t = 0; t < N; ++t) {
+            const u32 from = off[t] - (u32)__mul24(max(0, over + row(t)), (int)stride) * (u32)sizeof(T);
+            const u32 to = (u32)__builtin_amdgcn_readfirstlane((int)((u32)(uintptr_t)tile + (wave_index() * N + t) * 1024));
+            asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(from), "s"(at), "s"(to) : "memory");
         }
     }
 };
+// this wave's loads have arrived, then everyone's
+__device__ __forceinline__ void at_arrive() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+// Rows of a tile that nobody may see become zeros: a masked row may hold anything, also NaN, and must not reach a product.
+template <typename T, int DP> __device__ __forceinline__ void at_blank(T* tile, u64 bits) {
+    constexpr int CH = DP / 8;
+    for (int e = threadIdx.x; e < AT_TILE * CH; e += AT_BLOCK)
+        if (!((bits >> (e / CH)) & 1)) *(V8<T>*)(tile + e * 8) = V8<T>{};
+}
 __device__ __forceinline__ u64 read_lane(u64 x, int lane) {
     return ((u64)(u32)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32) | (u32)__builtin_amdgcn_readlane((int)x, lane);
 }
-__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 // A fragment: rows row0 + l % 32, dims 16 s + 8 (l / 32) + j
 template <typename T, int DP> __device__ __forceinline__ V8<T> at_rows(T* tile, int row0, int s) {
     const int l = threadIdx.x & 63;
@@ -206,33 +217,46 @@ __device__ __forceinline__ void at_hide(f32x16& s, u32 seen) {
         if (!((seen >> crow(i, 0)) & 1)) s[i] = -__builtin_inff();
 }
 
-// Runs `step(k0, bits)` for every tile of 64 keys in [0, end) that shows any key, with the tile's K and V in LDS; by the whole block.
+// Runs `step(k0, bits, K, V)` for every tile of 64 keys in [0, end) that shows any key, with the tile's K and V in LDS; by the whole block.
+// tiles: at_stages of [K, V][AT_TILE][DP].
 template <typename T, int DP, typename F>
-__device__ __forceinline__ void at_for_tiles(const AttnParams& p, int b, int h, int end, T* kt, T* vt, F&& step) {
-    AtTileIn<T, DP> kr((const T*)p.k + b * p.k_b + h * p.k_h, p.k_l, end, p.D), vr((const T*)p.v + b * p.v_b + h * p.v_h, p.v_l, end, p.D);
-    const bool whole = p.D == DP;
+__device__ __forceinline__ void at_for_tiles(const AttnParams& p, int b, int h, int end, T* tiles, F&& step) {
+    constexpr int S = at_stages(sizeof(T), DP), SIZE = AT_TILE * DP;
+    const AtStream<T, DP> ks((const T*)p.k + b * p.k_b + h * p.k_h, p.k_l, end, p.D), vs((const T*)p.v + b * p.v_b + h * p.v_h, p.v_l, end, p.D);
     for (int base = 0; base < end; base += 64 * AT_TILE) {
         const u64 words = at_words(p, b, base, end);
         u64 left = __ballot(words != 0);                                   // the same in every wave
         if (!left) continue;
-        int t = __builtin_ctzll(left);
-        kr.fetch(base + t * AT_TILE);
-        vr.fetch(base + t * AT_TILE);
+        int t = __builtin_ctzll(left), slot = 0;
+        __syncthreads();                                                   // (the readers of the 4096 keys before are done)
+        ks.load(base + t * AT_TILE, tiles);
+        vs.load(base + t * AT_TILE, tiles + SIZE);
         while (true) {
             const int k0 = base + t * AT_TILE;
             const u64 bits = read_lane(words, t);
+            T *kt = tiles + slot * 2 * SIZE, *vt = kt + SIZE;
             left &= left - 1;
-            __syncthreads();                                               // (the last step's readers are done)
-            kr.put(kt, bits, whole);
-            vr.put(vt, bits, whole);
-            __syncthreads();
-            if (left) {
+            at_arrive();                                                   // (also: the other slot has been read by every wave)
+            auto next = [&]() {
+                if (!left) return;
                 t = __builtin_ctzll(left);
-                kr.fetch(base + t * AT_TILE);
-                vr.fetch(base + t * AT_TILE);
+                if (S == 2) slot ^= 1;
+                ks.load(base + t * AT_TILE, tiles + slot * 2 * SIZE);
+                vs.load(base + t * AT_TILE, tiles + slot * 2 * SIZE + SIZE);
+            };
+            if (S == 2) next();
+            if (bits != ~0ull) {
+                at_blank<T, DP>(kt, bits);
+                at_blank<T, DP>(vt, bits);
+                __syncthreads();
             }
-            step(k0, bits);
-            if (!left) break;
+            const bool last = S == 2 ? k0 == base + t * AT_TILE : !left;
+            step(k0, bits, kt, vt);
+            if (last) break;
+            if (S == 1) {
+                __syncthreads();
+                next();
+            }
         }
     }
 }
@@ -306,9 +330,8 @@ __device__ __forceinline__ float at_norm(float sum) { return sum > 0.0f ? 1.0f /
 template <typename T, int DP, bool KEEP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_attn_forward_kernel(const AttnParams p) {
     extern __shared__ __align__(16) unsigned char at_lds[];
-    T* kt = (T*)at_lds;
-    T* vt = kt + AT_TILE * DP;
-    float* lut = (float*)(vt + AT_TILE * DP);
+    T* tiles = (T*)at_lds;
+    float* lut = (float*)(tiles + at_stages(sizeof(T), DP) * 2 * AT_TILE * DP);
     const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5;
     const int start = at_start(p, b);
     const int q = blockIdx.x * AT_COLS + wave * 32 + (l & 31);
@@ -327,7 +350,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     f32x16 acc[DP / 32] = {};
     float m = -__builtin_inff(), sum = 0.0f;
     const float c = p.scale * LOG2E;
-    at_for_tiles<T, DP>(p, b, h, end, kt, vt, [&](int k0, u64 bits) {
+    at_for_tiles<T, DP>(p, b, h, end, tiles, [&](int k0, u64 bits, T* kt, T* vt) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const u32 seen = (u32)(bits >> (32 * t));
@@ -528,9 +551,8 @@ __device__ __forceinline__ void at_diagonals(const f32x16& s, float* skew, float
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_attn_dq_kernel(const AttnParams p) {
     extern __shared__ __align__(16) unsigned char at_lds[];
-    T* kt = (T*)at_lds;
-    T* vt = kt + AT_TILE * DP;
-    float* lut = (float*)(vt + AT_TILE * DP);
+    T* tiles = (T*)at_lds;
+    float* lut = (float*)(tiles + at_stages(sizeof(T), DP) * 2 * AT_TILE * DP);
     const int n_lut = at_lut_size(p.sat);
     float* hist = lut + n_lut;                                             // [4 waves][n_lut] sums of dS by distance
     float* skew = hist + 4 * n_lut;                                        // [4 waves][32][32]
@@ -565,7 +587,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     f32x16 acc[DP / 32] = {};
     float far_lo = 0.0f, far_hi = 0.0f;
     const float c = p.scale * LOG2E;
-    at_for_tiles<T, DP>(p, b, h, end, kt, vt, [&](int k0, u64 bits) {
+    at_for_tiles<T, DP>(p, b, h, end, tiles, [&](int k0, u64 bits, T* kt, T* vt) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int row0 = k0 + 32 * t;
@@ -648,10 +670,10 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dtable_kernel(const float*
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_attn_dkv_kernel(const AttnParams p) {
     extern __shared__ __align__(16) unsigned char at_lds[];
-    T* qt = (T*)at_lds;
-    T* gt = qt + AT_TILE * DP;
-    float* rows = (float*)(gt + AT_TILE * DP);                             // [2][AT_TILE]: log2-sum, D
-    float* lut = rows + 2 * AT_TILE;
+    constexpr int S = at_stages(sizeof(T), DP), SIZE = AT_TILE * DP;
+    T* tiles = (T*)at_lds;                                                 // [S][Q, dO][AT_TILE][DP]
+    float* stats = (float*)(tiles + S * 2 * SIZE);                          // [S][log2-sum, D][AT_TILE]
+    float* lut = stats + S * 2 * AT_TILE;
     const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5;
     const int start = at_start(p, b);
     const int key0 = blockIdx.x * AT_COLS, key = key0 + wave * 32 + (l & 31);
@@ -676,27 +698,33 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const bool any = __syncthreads_or(seen);                               // (also the barrier behind at_lut)
     if (!any) first = p.Lq;
     first = first / AT_TILE * AT_TILE;
-    AtTileIn<T, DP> qr(qb, p.q_l, p.Lq, p.D), gr(gb, p.do_l, p.Lq, p.D);
-    if (first < p.Lq) {
-        qr.fetch(first);
-        gr.fetch(first);
-    }
+    const AtStream<T, DP> qs(qb, p.q_l, p.Lq, p.D), gs(gb, p.do_l, p.Lq, p.D);
+    float mine = 0.0f;                                                     // thread i: entry i of the next tile's statistics
+    auto fetch = [&](int q0, int slot) {
+        qs.load(q0, tiles + slot * 2 * SIZE);
+        gs.load(q0, tiles + slot * 2 * SIZE + SIZE);
+        if (threadIdx.x < 2 * AT_TILE) {
+            const int i = threadIdx.x % AT_TILE;
+            const bool in = q0 + i < p.Lq, d = threadIdx.x >= AT_TILE;
+            mine = in ? (d ? p.drow : p.lse)[srow + q0 + i] : 0.0f;
+            // rows behind the last and rows that saw nothing: P = exp2(s - inf) = 0
+            if (!d && (!in || mine == -__builtin_inff())) mine = __builtin_inff();
+            stats[slot * 2 * AT_TILE + threadIdx.x] = mine;
+        }
+    };
+    int slot = 0;
+    if (first < p.Lq) fetch(first, 0);
     for (int q0 = first; q0 < p.Lq; q0 += AT_TILE) {
-        __syncthreads();
-        const u64 bits = q0 + AT_TILE <= p.Lq ? ~0ull : (1ull << (p.Lq - q0)) - 1;
-        qr.put(qt, bits, p.D == DP);
-        gr.put(gt, bits, p.D == DP);
-        if (threadIdx.x < AT_TILE) {
-            const bool in = q0 + (int)threadIdx.x < p.Lq;
-            const float e = in ? p.lse[srow + q0 + threadIdx.x] : -__builtin_inff();
-            rows[threadIdx.x] = e == -__builtin_inff() ? __builtin_inff() : e;
-            rows[AT_TILE + threadIdx.x] = in ? p.drow[srow + q0 + threadIdx.x] : 0.0f;
+        T *qt = tiles + slot * 2 * SIZE, *gt = qt + SIZE;
+        const float* rows = stats + slot * 2 * AT_TILE;
+        at_arrive();
+        if (S == 2 && q0 + AT_TILE < p.Lq) fetch(q0 + AT_TILE, slot ^ 1);
+        if (q0 + AT_TILE > p.Lq) {
+            at_blank<T, DP>(qt, (1ull << (p.Lq - q0)) - 1);
+            at_blank<T, DP>(gt, (1ull << (p.Lq - q0)) - 1);
+            __syncthreads();
         }
-        __syncthreads();
-        if (q0 + AT_TILE < p.Lq) {
-            qr.fetch(q0 + AT_TILE);
-            gr.fetch(q0 + AT_TILE);
-        }
+        if (S == 2) slot ^= 1;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x16 s = {}, dp = {};
@@ -719,6 +747,10 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
                     dv[dt] = mma(at_cols<T, DP>(gt, 32 * t, g, dt), at_pack<T>(s, g), dv[dt]);
                     dk[dt] = mma(at_cols<T, DP>(qt, 32 * t, g, dt), at_pack<T>(dp, g), dk[dt]);
                 }
+        }
+        if (S == 1) {
+            __syncthreads();
+            if (q0 + AT_TILE < p.Lq) fetch(q0 + AT_TILE, 0);
         }
     }
     if (!live) return;

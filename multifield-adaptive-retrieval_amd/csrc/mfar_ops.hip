@@ -140,19 +140,20 @@ template <typename T, int DP> int attention_forward(const AttnParams& p, const A
             if (p.out_lo) return attention_few<T, DP, true>(p, sp, st);
         return attention_few<T, DP, false>(p, sp, st);
     }
-    const size_t lds = 2ull * AT_TILE * DP * sizeof(T) + lut_bytes(p);
+    const size_t lds = at_stages(sizeof(T), DP) * 2ull * AT_TILE * DP * sizeof(T) + lut_bytes(p);
     const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
     if constexpr (sizeof(T) == 2)
         if (p.out_lo) return launch<mfar_attn_forward_kernel<T, DP, true>>("mfar_attn_forward_kernel", grid, lds, st, p);
     return launch<mfar_attn_forward_kernel<T, DP, false>>("mfar_attn_forward_kernel", grid, lds, st, p);
 }
 template <typename T, int DP> int attention_backward(const AttnParams& p, float* dtable, hipStream_t st) {
-    const size_t tiles = 2ull * AT_TILE * DP * sizeof(T);
+    constexpr int S = at_stages(sizeof(T), DP);
+    const size_t tiles = S * 2ull * AT_TILE * DP * sizeof(T);
     const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
     int rc = launch<mfar_attn_dq_kernel<T, DP>>("mfar_attn_dq_kernel", grid, tiles + lut_bytes(p) * (p.dpart ? 5 : 1) + (p.dpart ? 4 * 1024 * 4 : 0), st, p);
     if (rc != MFAR_OK) return rc;
     if (p.Lk) {
-        rc = launch<mfar_attn_dkv_kernel<T, DP>>("mfar_attn_dkv_kernel", dim3(cdiv(p.Lk, AT_COLS), p.H, p.B), tiles + 2 * AT_TILE * 4 + lut_bytes(p), st, p);
+        rc = launch<mfar_attn_dkv_kernel<T, DP>>("mfar_attn_dkv_kernel", dim3(cdiv(p.Lk, AT_COLS), p.H, p.B), tiles + S * 2 * AT_TILE * 4 + lut_bytes(p), st, p);
         if (rc != MFAR_OK) return rc;
     }
     if (p.dpart) {
