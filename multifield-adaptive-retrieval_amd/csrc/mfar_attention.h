@@ -20,7 +20,7 @@
 #define AT_BLOCK 256      // 4 waves, 32 query (key) columns each
 #define AT_COLS 128
 #define AT_TILE 64        // keys (queries) staged in LDS per step
-#define AT_MAX_BORDERS 128
+#define AT_MAX_SAT 1023
 #define AT_MAX_STRIDE (1 << 22)
 // The running maximum of the softmax follows a tile's only when that is 2^8 over it: probabilities stay under 256 (fp16 holds them as exactly as
 // those under 1), and the accumulated output is hardly ever rescaled.
@@ -40,21 +40,16 @@ struct AttnParams {
     const int* start_ptr;        // [B] position of the first query among the keys, or NULL
     float *lse, *drow;           // [B, H, Lq], log2 units
     float* dpart;                // [blocks, H, n_buckets] partial bias gradients, or NULL
-    int start, B, Lq, Lk, H, D, causal, n_buckets, n_side, each, n_borders, sat;
+    int start, B, Lq, Lk, H, D, causal, n_buckets, n_side, sat;
     float scale;
-    int borders[AT_MAX_BORDERS]; // first distance of each shared bucket after the first
+    short first[129 * 2];        // first distance of each bucket of a side
+    unsigned char bucket[AT_MAX_SAT + 1];   // of the distances 0 .. sat
 };
 
 __device__ __forceinline__ int attn_bucket(const AttnParams& p, int delta) {
-    int far = p.causal ? (delta < 0 ? -delta : 0) : (delta < 0 ? -delta : delta);
-    int b = far;
-    if (far >= p.each) {
-        b = p.each;
-        for (int j = 0; j < p.n_borders; ++j) b += far >= p.borders[j] ? 1 : 0;
-    }
-    return b + ((delta > 0 && !p.causal) ? p.n_side : 0);
+    const int far = p.causal ? max(-delta, 0) : abs(delta);
+    return p.bucket[min(far, p.sat)] + ((delta > 0 && !p.causal) ? p.n_side : 0);
 }
-
 // (a position from device memory is kept where sums of positions fit 32 bits)
 __device__ __forceinline__ int at_start(const AttnParams& p, int b) { return p.start_ptr ? min(max(p.start_ptr[b], -(1 << 30)), 1 << 30) : p.start; }
 
@@ -218,19 +213,23 @@ __device__ __forceinline__ void at_hide(f32x16& s, u32 seen) {
 }
 
 // Runs `step(k0, bits, K, V)` for every tile of 64 keys in [0, end) that shows any key, with the tile's K and V in LDS; by the whole block.
-// tiles: at_stages of [K, V][AT_TILE][DP].
-template <typename T, int DP, typename F>
-__device__ __forceinline__ void at_for_tiles(const AttnParams& p, int b, int h, int end, T* tiles, F&& step) {
+// tiles: at_stages of [K, V][AT_TILE][DP].  `ahead()` is run once, while the first tile is on its way.
+template <typename T, int DP, typename A, typename F>
+__device__ __forceinline__ void at_for_tiles(const AttnParams& p, int b, int h, int end, T* tiles, A&& ahead, F&& step) {
     constexpr int S = at_stages(sizeof(T), DP), SIZE = AT_TILE * DP;
     const AtStream<T, DP> ks((const T*)p.k + b * p.k_b + h * p.k_h, p.k_l, end, p.D), vs((const T*)p.v + b * p.v_b + h * p.v_h, p.v_l, end, p.D);
+    if (end <= 0) ahead();
     for (int base = 0; base < end; base += 64 * AT_TILE) {
         const u64 words = at_words(p, b, base, end);
         u64 left = __ballot(words != 0);                                   // the same in every wave
+        int t = left ? __builtin_ctzll(left) : 0, slot = 0;
+        if (base) __syncthreads();                                         // (the readers of the 4096 keys before are done)
+        if (left) {
+            ks.load(base + t * AT_TILE, tiles);
+            vs.load(base + t * AT_TILE, tiles + SIZE);
+        }
+        if (base == 0) ahead();
         if (!left) continue;
-        int t = __builtin_ctzll(left), slot = 0;
-        __syncthreads();                                                   // (the readers of the 4096 keys before are done)
-        ks.load(base + t * AT_TILE, tiles);
-        vs.load(base + t * AT_TILE, tiles + SIZE);
         while (true) {
             const int k0 = base + t * AT_TILE;
             const u64 bits = read_lane(words, t);
@@ -342,15 +341,16 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
         const int last = start + min(p.Lq, ((int)blockIdx.x + 1) * AT_COLS);      // one past the last query's position
         end = min(end, max(last, 0));
     }
-    at_lut(p, lut, h);
     const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
     V8<T> qf[DP / 16];
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) qf[s] = at_load<T>(qrow, live, s, p.D);
     f32x16 acc[DP / 32] = {};
     float m = -__builtin_inff(), sum = 0.0f;
     const float c = p.scale * LOG2E;
-    at_for_tiles<T, DP>(p, b, h, end, tiles, [&](int k0, u64 bits, T* kt, T* vt) {
+    at_for_tiles<T, DP>(p, b, h, end, tiles, [&]() {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) qf[s] = at_load<T>(qrow, live, s, p.D);
+        at_lut(p, lut, h);
+    }, [&](int k0, u64 bits, T* kt, T* vt) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const u32 seen = (u32)(bits >> (32 * t));
@@ -563,31 +563,31 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const int col = start + q, col_lo = start + (int)blockIdx.x * AT_COLS + wave * 32;
     int end = p.Lk;
     if (p.causal) end = min(end, max(start + min(p.Lq, ((int)blockIdx.x + 1) * AT_COLS), 0));
-    at_lut(p, lut, h);
-    if (p.dpart)
-        for (int i = threadIdx.x; i < 4 * n_lut; i += AT_BLOCK) hist[i] = 0.0f;
     const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
     const T* grow = (const T*)p.dout + b * p.do_b + (long long)q * p.do_l + h * p.do_h;
-    const long long orow = (((long long)b * p.Lq + q) * p.H + h) * p.D;
+    const long long orow = (((long long)b * p.Lq + q) * p.H + h) * p.D, srow = ((long long)b * p.H + h) * p.Lq + q;
     V8<T> qf[DP / 16], gf[DP / 16];
-    float dsum = 0.0f;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-        qf[s] = at_load<T>(qrow, live, s, p.D);
-        gf[s] = at_load<T>(grow, live, s, p.D);
-        const V8<T> o = at_load<T>((const T*)p.o + orow, live, s, p.D), lo = at_load<T>((const T*)p.o_lo + orow, live && p.o_lo, s, p.D);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dsum = __builtin_fmaf((float)gf[s][j], (float)o[j] + (float)lo[j], dsum);
-    }
-    dsum = sum_halves(dsum);
-    const long long srow = ((long long)b * p.H + h) * p.Lq + q;
-    float lse = live ? p.lse[srow] : 0.0f;
-    if (!live || lse == -__builtin_inff()) lse = __builtin_inff();          // no keys: P = exp2(-inf) = 0 everywhere
-    if (live && half == 0) p.drow[srow] = dsum;
+    float dsum = 0.0f, lse = 0.0f;
     f32x16 acc[DP / 32] = {};
     float far_lo = 0.0f, far_hi = 0.0f;
     const float c = p.scale * LOG2E;
-    at_for_tiles<T, DP>(p, b, h, end, tiles, [&](int k0, u64 bits, T* kt, T* vt) {
+    at_for_tiles<T, DP>(p, b, h, end, tiles, [&]() {
+        if (live) lse = p.lse[srow];
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            qf[s] = at_load<T>(qrow, live, s, p.D);
+            gf[s] = at_load<T>(grow, live, s, p.D);
+            const V8<T> o = at_load<T>((const T*)p.o + orow, live, s, p.D), lo = at_load<T>((const T*)p.o_lo + orow, live && p.o_lo, s, p.D);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dsum = __builtin_fmaf((float)gf[s][j], (float)o[j] + (float)lo[j], dsum);
+        }
+        at_lut(p, lut, h);
+        if (p.dpart)
+            for (int i = threadIdx.x; i < 4 * n_lut; i += AT_BLOCK) hist[i] = 0.0f;
+        dsum = sum_halves(dsum);
+        if (!live || lse == -__builtin_inff()) lse = __builtin_inff();      // no keys: P = exp2(-inf) = 0 everywhere
+        if (live && half == 0) p.drow[srow] = dsum;
+    }, [&](int k0, u64 bits, T* kt, T* vt) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int row0 = k0 + 32 * t;
@@ -640,13 +640,11 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
         // a bucket holds the distances [lo, hi) of one side
         float* to = p.dpart + ((long long)(b * gridDim.x + blockIdx.x) * p.H + h) * p.n_buckets;
         for (int n = threadIdx.x; n < p.n_buckets; n += AT_BLOCK) {
-            const bool ahead = n >= p.n_side;
-            const int m = n - (ahead ? p.n_side : 0), top = p.sat + AT_EDGE + 1;
-            int lo = m <= p.each ? m : p.borders[m - p.each - 1];
-            const int hi = m < p.each ? m + 1 : (m == p.n_side - 1 ? top : p.borders[m - p.each]);
-            if (ahead && lo == 0) lo = 1;                                  // distance 0 counts as behind
+            const bool front = n >= p.n_side;
+            const int m = n - (front ? p.n_side : 0);
+            const int lo = max((int)p.first[m], front ? 1 : 0), hi = m == p.n_side - 1 ? p.sat + AT_EDGE + 1 : p.first[m + 1];   // (distance 0 counts as behind)
             float t = 0.0f;
-            for (int d = lo; d < hi; ++d) t += hist[(ahead ? d : -d) + p.sat + AT_EDGE];
+            for (int d = lo; d < hi; ++d) t += hist[(front ? d : -d) + p.sat + AT_EDGE];
             to[n] = t;
         }
     }
@@ -680,23 +678,13 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const bool live = key < p.Lk;
     const bool seen = live && (!p.mask || p.mask[(long long)b * p.mask_b + key] != 0);
     const int col_lo = key0 + wave * 32;
-    at_lut(p, lut, h);
-    const T* krow = (const T*)p.k + b * p.k_b + (long long)key * p.k_l + h * p.k_h;
-    const T* vrow = (const T*)p.v + b * p.v_b + (long long)key * p.v_l + h * p.v_h;
-    V8<T> kf[DP / 16], vf[DP / 16];
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-        kf[s] = at_load<T>(krow, seen, s, p.D);
-        vf[s] = at_load<T>(vrow, seen, s, p.D);
-    }
     f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
     const float c = p.scale * LOG2E;
     const T* qb = (const T*)p.q + b * p.q_b + h * p.q_h;
     const T* gb = (const T*)p.dout + b * p.do_b + h * p.do_h;
     const long long srow = ((long long)b * p.H + h) * p.Lq;
     int first = p.causal ? max(0, key0 - start) : 0;                       // the first query that sees the block's first key
-    const bool any = __syncthreads_or(seen);                               // (also the barrier behind at_lut)
-    if (!any) first = p.Lq;
+    if (!__syncthreads_or(seen)) first = p.Lq;
     first = first / AT_TILE * AT_TILE;
     const AtStream<T, DP> qs(qb, p.q_l, p.Lq, p.D), gs(gb, p.do_l, p.Lq, p.D);
     float mine = 0.0f;                                                     // thread i: entry i of the next tile's statistics
@@ -714,6 +702,15 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     };
     int slot = 0;
     if (first < p.Lq) fetch(first, 0);
+    const T* krow = (const T*)p.k + b * p.k_b + (long long)key * p.k_l + h * p.k_h;
+    const T* vrow = (const T*)p.v + b * p.v_b + (long long)key * p.v_l + h * p.v_h;
+    V8<T> kf[DP / 16], vf[DP / 16];
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+        kf[s] = at_load<T>(krow, seen, s, p.D);
+        vf[s] = at_load<T>(vrow, seen, s, p.D);
+    }
+    at_lut(p, lut, h);
     for (int q0 = first; q0 < p.Lq; q0 += AT_TILE) {
         T *qt = tiles + slot * 2 * SIZE, *gt = qt + SIZE;
         const float* rows = stats + slot * 2 * AT_TILE;

@@ -110,9 +110,14 @@ AttnParams attention_params(const mfar_attention* a) {
     p.do_b = a->do_b, p.do_l = a->do_l, p.do_h = a->do_h;
     p.table = a->table, p.mask = a->key_mask, p.mask_b = a->mask_b, p.start_ptr = a->q_start_each, p.start = a->q_start, p.lse = a->lse;
     p.B = a->B, p.Lq = a->Lq, p.Lk = a->Lk, p.H = a->H, p.D = a->D, p.causal = a->causal != 0, p.scale = a->scale;
-    p.n_buckets = a->n_buckets, p.n_side = a->causal ? a->n_buckets : a->n_buckets / 2, p.each = p.n_side / 2, p.n_borders = a->n_borders;
-    for (int j = 0; j < a->n_borders; ++j) p.borders[j] = a->borders[j];
-    p.sat = a->n_borders ? a->borders[a->n_borders - 1] : p.each;
+        p.n_buckets = a->n_buckets, p.n_side = a->causal ? a->n_buckets : a->n_buckets / 2;
+    const int each = p.n_side / 2;
+    p.sat = a->n_borders ? a->borders[a->n_borders - 1] : each;
+    for (int m = 0; m < p.n_side; ++m) p.first[m] = (short)(m <= each ? m : a->borders[m - each - 1]);
+    for (int d = 0, m = 0; d <= p.sat; ++d) {
+        while (m + 1 < p.n_side && d >= p.first[m + 1]) ++m;
+        p.bucket[d] = (unsigned char)m;
+    }
     return p;
 }
 int64_t drow_bytes(const mfar_attention* a) { return ((int64_t)a->B * a->H * a->Lq * 4 + 15) / 16 * 16; }
