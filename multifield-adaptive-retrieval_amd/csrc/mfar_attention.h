@@ -89,12 +89,16 @@ template <typename T, int DP> struct AtStream {
     __device__ __forceinline__ void load(int r0, T* tile) const {
         const u64 address = (u64)(uintptr_t)(base + (long long)r0 * stride);
         const u64 at = ((u64)(u32)__builtin_amdgcn_readfirstlane((int)(address >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)address);
-        const int over = r0 - (n - 1);
+        const u32 to = (u32)__builtin_amdgcn_readfirstlane((int)((u32)(uintptr_t)tile + wave_index() * N * 1024));
+        auto go = [&](u32 from, int t) {
+            asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(from), "s"(at), "s"(to + t * 1024) : "memory");
+        };
+        if (r0 + AT_TILE <= n) {
 #pragma unroll
-        for (int t = 0; t < N; ++t) {
-            const u32 from = off[t] - (u32)__mul24(max(0, over + row(t)), (int)stride) * (u32)sizeof(T);
-            const u32 to = (u32)__builtin_amdgcn_readfirstlane((int)((u32)(uintptr_t)tile + (wave_index() * N + t) * 1024));
-            asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(from), "s"(at), "s"(to) : "memory");
+            for (int t = 0; t < N; ++t) go(off[t], t);
+        } else {
+#pragma unroll
+            for (int t = 0; t < N; ++t) go(off[t] - (u32)__mul24(max(0, r0 + row(t) - (n - 1)), (int)stride) * (u32)sizeof(T), t);
         }
     }
 };
@@ -268,20 +272,20 @@ __device__ __forceinline__ void at_lut(const AttnParams& p, float* lut, int h) {
     for (int i = threadIdx.x; i < at_lut_size(p.sat); i += AT_BLOCK)
         lut[i] = p.table[(long long)attn_bucket(p, i - p.sat - AT_EDGE) * p.H + h] * LOG2E;
 }
-// s2 = s * c + bias for this lane's 16 elements of a 32 x 32 tile, places behind the query -inf when causal.
+// s2 - off = s * c + bias - off for this lane's 16 elements of a 32 x 32 tile, places behind the query -inf when causal.
 // SIGN = +1: the lane's column is a query at position `col`, rows are keys from row0; -1: the column is a key, rows are query positions from row0.
 template <int SIGN>
-__device__ __forceinline__ void at_bias(f32x16& s, const float* lut, int sat, float c, int row0, int col, int col_lo, bool causal) {
+__device__ __forceinline__ void at_bias(f32x16& s, const float* lut, int sat, float c, int row0, int col, int col_lo, bool causal, float off) {
     const int half = (threadIdx.x & 63) >> 5;
     const int lo = SIGN > 0 ? row0 - col_lo - 31 : col_lo - row0 - 31, hi = lo + 62;      // key - query over the tile
     if (lo >= sat || hi <= -sat) {
-        const float add = lut[lo >= sat ? 2 * (sat + AT_EDGE) : 0];
+        const float add = lut[lo >= sat ? 2 * (sat + AT_EDGE) : 0] - off;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], c, add);
     } else {
         const float* at = lut + (SIGN > 0 ? row0 + 4 * half - col : col - row0 - 4 * half) + sat + AT_EDGE;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], c, at[SIGN * crow(i, 0)]);
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], c, at[SIGN * crow(i, 0)] - off);
     }
     if (causal && hi > 0) {
         const int edge = SIGN > 0 ? col - row0 - 4 * half : row0 + 4 * half - col;         // the last visible row / minus the first
@@ -291,35 +295,55 @@ __device__ __forceinline__ void at_bias(f32x16& s, const float* lut, int sat, fl
     }
 }
 
-// One 32 x 32 tile of scores into the running softmax: maximum m, this half's part of the sum, and O' += V' P' with the rows from row0 of vt.
-template <typename T, int DP, bool KEEP>
-__device__ __forceinline__ void at_softmax(f32x16& s, T* vt, int row0, float& m, float& sum, f32x16* acc) {
+// Running softmax of a lane's query.  Scores arrive as x = s2 - base (at_bias takes the base off with the bias); the base moves to the tile's maximum only
+// when that is 2^AT_SLACK over it, and at the first visible key (limit = -inf until then).
+struct AtSoftmax {
+    float base = 0.0f, limit = -__builtin_inff(), sum = 0.0f;               // sum: this half's part
+};
+// N tiles of 32 x 32 scores into the softmax and O' += V' P' with the rows of vt.
+template <typename T, int DP, bool KEEP, int N>
+__device__ __forceinline__ void at_softmax(f32x16 (&s)[N], T* vt, AtSoftmax& m, f32x16* acc) {
     float top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
     top = max_halves(top);
-    if (__any(top > m + AT_SLACK)) {                                        // (m = -inf at first: any number is over it)
-        const float up = fmaxf(top, m), keep = up == -__builtin_inff() ? 1.0f : exp2_fast(m - up);
-        m = up;
-        sum *= keep;
+    if (__any(top > m.limit)) {
+        const float up = top > m.limit ? top : 0.0f, keep = m.limit > 0.0f ? exp2_fast(-up) : 0.0f;   // (before the first key there is nothing to keep)
+        m.base += up;
+        if (top > m.limit) m.limit = AT_SLACK;
+        m.sum *= keep;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= keep;
-    }
-    const float base = m == -__builtin_inff() ? 0.0f : m;                   // nothing visible so far: exp2(-inf - 0) = 0
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        s[i] = exp2_fast(s[i] - base);
-        sum += s[i];
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] -= up;
     }
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int t = 0; t < N; ++t) {
+        float part[2] = {};
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const V8<T> vf = at_cols<T, DP>(vt, row0, g, dt);
-            acc[dt] = mma(vf, at_pack<T>(s, g), acc[dt]);
-            if (KEEP) acc[dt] = mma(vf, at_pack_lo<T>(s, g), acc[dt]);
+        for (int i = 0; i < 16; ++i) {
+            s[t][i] = exp2_fast(s[t][i]);
+            part[i & 1] += s[t][i];
         }
+        m.sum += part[0] + part[1];
+        if (sizeof(T) == 2) __builtin_amdgcn_s_setprio(1);                 // (matrix work first: the other waves' exponentials fill the gaps; 3 % at 8 x 4096)
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const V8<T> vf = at_cols<T, DP>(vt, 32 * t, g, dt);
+                acc[dt] = mma(vf, at_pack<T>(s[t], g), acc[dt]);
+                if (KEEP) acc[dt] = mma(vf, at_pack_lo<T>(s[t], g), acc[dt]);
+            }
+        if (sizeof(T) == 2) __builtin_amdgcn_s_setprio(0);
+    }
 }
+// log2-sum of a query: -inf if it saw nothing
+__device__ __forceinline__ float at_lse(float base, float sum) { return sum == 0.0f ? -__builtin_inff() : base + __log2f(sum); }
 
 __device__ __forceinline__ float at_norm(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }   // no keys: zeros; NaN stays
 
@@ -344,25 +368,26 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
     V8<T> qf[DP / 16];
     f32x16 acc[DP / 32] = {};
-    float m = -__builtin_inff(), sum = 0.0f;
+    AtSoftmax m;
     const float c = p.scale * LOG2E;
     at_for_tiles<T, DP>(p, b, h, end, tiles, [&]() {
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) qf[s] = at_load<T>(qrow, live, s, p.D);
         at_lut(p, lut, h);
     }, [&](int k0, u64 bits, T* kt, T* vt) {
+        f32x16 s[2] = {};
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[t] = mma(at_rows<T, DP>(kt, 32 * t, d), qf[d], s[t]);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const u32 seen = (u32)(bits >> (32 * t));
-            f32x16 s = {};
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d) s = mma(at_rows<T, DP>(kt, 32 * t, d), qf[d], s);
-            at_bias<1>(s, lut, p.sat, c, k0 + 32 * t, col, col_lo, p.causal != 0);
-            if (seen != ~0u) at_hide(s, seen);
-            at_softmax<T, DP, KEEP>(s, vt, 32 * t, m, sum, acc);
+            at_bias<1>(s[t], lut, p.sat, c, k0 + 32 * t, col, col_lo, p.causal != 0, m.base);
+            if ((u32)(bits >> (32 * t)) != ~0u) at_hide(s[t], (u32)(bits >> (32 * t)));
         }
+        at_softmax<T, DP, KEEP, 2>(s, vt, m, acc);
     });
-    sum = sum_halves(sum);
+    const float sum = sum_halves(m.sum);
     if (!live) return;
     const float f = at_norm(sum);
     const long long row = ((long long)b * p.Lq + q) * p.H + h;
@@ -374,7 +399,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
             for (int i = 0; i < 16; ++i) acc[dt][i] = acc[dt][i] * f - (float)(T)(acc[dt][i] * f);
         at_store<T, DP>((T*)p.out_lo + row * p.D, acc, 1.0f, p.D);
     }
-    if (p.lse && half == 0) p.lse[((long long)b * p.H + h) * p.Lq + q] = sum == 0.0f ? -__builtin_inff() : m + __log2f(sum);
+    if (p.lse && half == 0) p.lse[((long long)b * p.H + h) * p.Lq + q] = at_lse(m.base, sum);
 }
 
 // ---- forward, up to 32 queries (short texts, a decoder's next token): the work is in the keys ------------------------------------------------
@@ -431,14 +456,14 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     at_lut(p, lut, h);
     __syncthreads();
     f32x16 acc[DP / 32] = {};
-    float m = -__builtin_inff(), sum = 0.0f;
+    AtSoftmax run;
     const float c = p.scale * LOG2E;
     while (k0 < end) {
         const u32 seen = (u32)__ballot(on);
         const int row0 = k0;
-        f32x16 s = {};
+        f32x16 s[1] = {};
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) s = mma(kf[d], qf[d], s);
+        for (int d = 0; d < DP / 16; ++d) s[0] = mma(kf[d], qf[d], s[0]);
 #pragma unroll
         for (int t = 0; t < NV; ++t) {
             const int r = (t * 64 + l) / CH;
@@ -449,14 +474,14 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (seen) {
-            at_bias<1>(s, lut, p.sat, c, row0, col, start, p.causal != 0);
-            if (seen != ~0u) at_hide(s, seen);
-            at_softmax<T, DP, KEEP>(s, vt, 0, m, sum, acc);
+            at_bias<1>(s[0], lut, p.sat, c, row0, col, start, p.causal != 0, run.base);
+            if (seen != ~0u) at_hide(s[0], seen);
+            at_softmax<T, DP, KEEP, 1>(s, vt, run, acc);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
-    sum = sum_halves(sum);
+    float m = run.limit > 0.0f ? run.base : -__builtin_inff(), sum = sum_halves(run.sum);
     __syncthreads();                                                       // (part lies where the V tiles were)
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
@@ -597,11 +622,11 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
                 s = mma(at_rows<T, DP>(kt, 32 * t, d), qf[d], s);
                 dp = mma(at_rows<T, DP>(vt, 32 * t, d), gf[d], dp);
             }
-            at_bias<1>(s, lut, p.sat, c, row0, col, col_lo, p.causal != 0);
+            at_bias<1>(s, lut, p.sat, c, row0, col, col_lo, p.causal != 0, lse);
             const u32 shown = (u32)(bits >> (32 * t));
             if (shown != ~0u) at_hide(s, shown);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i] - lse) * (dp[i] - dsum);
+            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i]) * (dp[i] - dsum);
             if (p.dpart) {
                 if (row0 - col_lo - 31 >= p.sat) {
 #pragma unroll
@@ -730,7 +755,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
                 s = mma(at_rows<T, DP>(qt, 32 * t, d), kf[d], s);
                 dp = mma(at_rows<T, DP>(gt, 32 * t, d), vf[d], dp);
             }
-            at_bias<-1>(s, lut, p.sat, c, start + q0 + 32 * t, key, col_lo, p.causal != 0);
+            at_bias<-1>(s, lut, p.sat, c, start + q0 + 32 * t, key, col_lo, p.causal != 0, 0.0f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = 32 * t + crow(i, half);
