@@ -78,6 +78,7 @@ int check_attention(const mfar_attention* a, bool backward) {
     if (!es) return bad("dtype must be F32, BF16 or F16");
     if (a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 1 || a->B > 65535 || a->H > 65535) return bad("B, Lq, Lk must be >= 0, H >= 1, B and H <= 65535");
     if (a->D < 8 || a->D > 128 || a->D % 8) return bad("D must be a multiple of 8, at most 128");
+    if (cdiv((int64_t)a->B * a->H, 8) * 8 * cdiv(std::max(a->Lq, a->Lk), AT_COLS) > 0x7fffffff) return bad("too many tiles for one launch");
     if (a->Lq > (1 << 30) || a->Lk > (1 << 30)) return bad("at most 2^30 queries and keys");
     if (a->q_start < -(1 << 30) || a->q_start > (1 << 30)) return bad("q_start out of range");
     if (a->n_buckets < 2 || a->n_buckets > 256 || (!a->causal && (a->n_buckets % 2 || a->n_buckets < 4))) return bad("n_buckets must be 2..256, even and >= 4 unless causal");
@@ -121,6 +122,12 @@ AttnParams attention_params(const mfar_attention* a) {
     return p;
 }
 int64_t drow_bytes(const mfar_attention* a) { return ((int64_t)a->B * a->H * a->Lq * 4 + 15) / 16 * 16; }
+// (behind the loop the tiles' memory takes the results on their way out)
+template <typename T, int DP> constexpr size_t tile_bytes() {
+    constexpr size_t n = at_stages(sizeof(T), DP) * 2ull * AT_TILE * DP * sizeof(T);
+    static_assert(n >= 4 * at_out_bytes<T, DP>());
+    return n;
+}
 size_t lut_bytes(const AttnParams& p) { return (size_t)(2 * (p.sat + AT_EDGE) + 1) * 4; }
 
 // Up to 32 queries take the kernel that divides the keys over waves and blocks; a block gets at least 8 tiles of 32 keys, and there are no more
@@ -139,30 +146,33 @@ template <typename T, int DP, bool KEEP> int attention_few(const AttnParams& p, 
         rc = launch<mfar_attn_join_kernel<T, KEEP>>("mfar_attn_join_kernel", dim3(cdiv((int64_t)p.B * p.Lq * p.H, 4)), 0, st, p, sp);
     return rc;
 }
+// blocks of 128 columns for every (batch, head), in groups of 8 (at_place)
+unsigned at_grid(const AttnParams& p, int64_t columns) { return (unsigned)(cdiv((int64_t)p.B * p.H, 8) * 8 * cdiv(columns, AT_COLS)); }
+
 template <typename T, int DP> int attention_forward(const AttnParams& p, const AttnSplit& sp, hipStream_t st) {
     if (sp.splits) {
         if constexpr (sizeof(T) == 2)
             if (p.out_lo) return attention_few<T, DP, true>(p, sp, st);
         return attention_few<T, DP, false>(p, sp, st);
     }
-    const size_t lds = at_stages(sizeof(T), DP) * 2ull * AT_TILE * DP * sizeof(T) + lut_bytes(p);
-    const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
+    const size_t lds = tile_bytes<T, DP>() + lut_bytes(p);
+    const dim3 grid(at_grid(p, p.Lq));
     if constexpr (sizeof(T) == 2)
         if (p.out_lo) return launch<mfar_attn_forward_kernel<T, DP, true>>("mfar_attn_forward_kernel", grid, lds, st, p);
     return launch<mfar_attn_forward_kernel<T, DP, false>>("mfar_attn_forward_kernel", grid, lds, st, p);
 }
 template <typename T, int DP> int attention_backward(const AttnParams& p, float* dtable, hipStream_t st) {
     constexpr int S = at_stages(sizeof(T), DP);
-    const size_t tiles = S * 2ull * AT_TILE * DP * sizeof(T);
-    const dim3 grid(cdiv(p.Lq, AT_COLS), p.H, p.B);
+    const size_t tiles = tile_bytes<T, DP>();
+    const dim3 grid(at_grid(p, p.Lq));
     int rc = launch<mfar_attn_dq_kernel<T, DP>>("mfar_attn_dq_kernel", grid, tiles + lut_bytes(p) * (p.dpart ? 5 : 1) + (p.dpart ? 4 * 1024 * 4 : 0), st, p);
     if (rc != MFAR_OK) return rc;
     if (p.Lk) {
-        rc = launch<mfar_attn_dkv_kernel<T, DP>>("mfar_attn_dkv_kernel", dim3(cdiv(p.Lk, AT_COLS), p.H, p.B), tiles + S * 2 * AT_TILE * 4 + lut_bytes(p), st, p);
+        rc = launch<mfar_attn_dkv_kernel<T, DP>>("mfar_attn_dkv_kernel", dim3(at_grid(p, p.Lk)), tiles + S * 2 * AT_TILE * 4 + lut_bytes(p), st, p);
         if (rc != MFAR_OK) return rc;
     }
     if (p.dpart) {
-        mfar_attn_dtable_kernel<<<p.H * p.n_buckets, AT_BLOCK, 0, st>>>(p.dpart, (int)(grid.x * grid.z), p.H, p.n_buckets, dtable);
+        mfar_attn_dtable_kernel<<<p.H * p.n_buckets, AT_BLOCK, 0, st>>>(p.dpart, (int)(cdiv(p.Lq, AT_COLS) * p.B), p.H, p.n_buckets, dtable);
         LAUNCHED("mfar_attn_dtable_kernel");
     }
     return MFAR_OK;
