@@ -542,13 +542,13 @@ int mfar_attention_backward(int device, const mfar_attention* a, void* stream); 
  * 8-bit products with a scale for each token (row of x) and each output channel.
  *   mfar_quantize_rows: scale[m] = max|x[m]| / 127, q[m] = rint(x[m] / scale[m]), ties to even; rows of q ldq bytes apart.  A row of zeros gets
  *   scale 0, a row with an infinity or NaN scale NaN and zeros.
- *   mfar_int8_linear: y = quantize_rows(x) wq' scaled by both scales (+ bias), rounded once to x's type.
- * x [M, K] rows ldx elements apart; wq [N, K] contiguous, 16-byte aligned; w_scale [N]; bias [N] fp32 or NULL; y [M, N] contiguous, of x's type.  K <= 131072.
+ *   mfar_int8_linear: y = quantize_rows(x) wq' scaled by both scales (+ bias), rounded once to y's type.
+ * x [M, K] rows ldx elements apart; wq [N, K] contiguous, 16-byte aligned; w_scale [N]; bias [N] fp32 or NULL; y [M, N] contiguous, of any of the three types.  K <= 131072.
  */
 int mfar_quantize_rows(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int8_t* q, int64_t ldq, float* scale, void* stream);
 int64_t mfar_int8_linear_workspace_bytes(int64_t M, int K, int N);
 int mfar_int8_linear(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int N, const int8_t* wq, const float* w_scale,
-                     const float* bias, void* y, void* workspace, int64_t workspace_bytes, void* stream);
+                     const float* bias, void* y, int y_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Distillation from a teacher's top scores: p = softmax(scores / tau) over a row's ids >= 0, q = softmax(student / tau) over its N columns;

@@ -292,10 +292,11 @@ extern "C" int64_t mfar_int8_linear_workspace_bytes(int64_t M, int K, int N) {
     return int8_weights_at(M, K) + (copies_weights(M, N, K) ? (int64_t)N * padded_k(K) : 0);
 }
 extern "C" int mfar_int8_linear(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int N, const int8_t* wq, const float* w_scale,
-                                const float* bias, void* y, void* workspace, int64_t workspace_bytes, void* stream) {
+                                const float* bias, void* y, int y_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
     int rc = check_rows(x, dtype, ldx, M, K);
     if (rc != MFAR_OK) return rc;
     if (N < 0 || N > (1 << 23)) return bad("N must be 0..2^23");
+    if (!type_size(y_dtype)) return bad("y_dtype must be F32, BF16 or F16");
     if (M == 0 || N == 0) return MFAR_OK;
     if (!wq || !w_scale || !y) return bad("NULL tensor");
     if (!aligned16(wq)) return bad("the weights must be 16-byte aligned");
@@ -315,8 +316,8 @@ extern "C" int mfar_int8_linear(int device, const void* x, int dtype, int64_t ld
     rc = FOR_TYPE(dtype, quantize_rows, x, ldx, M, K, xq, Kp, xs, 1, cp, st);
     if (rc != MFAR_OK) return rc;
     const Int8Params p = {(const signed char*)xq, w, xs, w_scale, bias, y, (long long)Kp, (long long)ldw,
-                          (int64_t)N * type_size(dtype) % 16 == 0 && aligned16(y), (int)M, N, K, (int)Kp};
-    return FOR_TYPE(dtype, int8_product, p, st);
+                          (int64_t)N * type_size(y_dtype) % 16 == 0 && aligned16(y), (int)M, N, K, (int)Kp};
+    return FOR_TYPE(y_dtype, int8_product, p, st);
 }
 
 extern "C" int64_t mfar_distill_workspace_bytes(int64_t T, int64_t N) {

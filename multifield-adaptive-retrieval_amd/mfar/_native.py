@@ -126,7 +126,7 @@ SIGNATURES = {
     "mfar_attention_backward": (_i, [_i, _c.POINTER(Attention), _vp]),
     "mfar_quantize_rows": (_i, [_i, _vp, _i, _i64, _i64, _i, _vp, _i64, _vp, _vp]),
     "mfar_int8_linear_workspace_bytes": (_i64, [_i64, _i, _i]),
-    "mfar_int8_linear": (_i, [_i, _vp, _i, _i64, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mfar_int8_linear": (_i, [_i, _vp, _i, _i64, _i64, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i64, _vp]),
     "mfar_distill_workspace_bytes": (_i64, [_i64, _i64]),
     "mfar_distill_forward": (_i, [_i, _vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _c.c_float, _vp, _vp, _vp, _vp, _i64, _vp]),
     "mfar_distill_backward": (_i, [_i, _vp, _i, _i64, _i64, _i64, _vp, _i, _c.c_float, _vp, _vp, _vp, _vp, _vp]),

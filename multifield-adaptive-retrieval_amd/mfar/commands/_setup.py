@@ -51,6 +51,9 @@ def build(flags: dict, freeze_encoder: bool = False) -> SimpleNamespace:
     model_id = f.get("model_path") or f["model_name"]
     tokenizer, encoder, _ = prepare_model(model_id, normalize=f["normalize"], with_decoder=False, freeze_encoder=freeze_encoder)
     encoder.to(device)
+    # MFAR_FUSED_ATTENTION=1: the gtr-t5 encoders run the fused relative-bias attention (training and encoding); other encoders refuse it
+    if os.environ.get("MFAR_FUSED_ATTENTION", "0") == "1":
+        encoder.use_fused_attention()
     corpus, vectors_dict, indices_dict = read_and_create_indices(f"{f['corpus']}/corpus", f["dataset_name"], field_info,
                                                                   f["temp_dir"], encoder)
     shared = ("lexical_index", "negative_sampling_params", "train_batch_size", "dev_batch_size", "train_max_length",

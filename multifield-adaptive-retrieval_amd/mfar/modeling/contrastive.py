@@ -14,6 +14,7 @@
     (`ShardedSearcher`); rank 0 writes the result lines.  The reference instead shards the queries over ranks and has every
     rank search the full corpus on its CPU (contrastive.py:184,200,207).  File names and formats are unchanged.
 """
+import contextlib
 import json
 import os
 import shutil
@@ -149,9 +150,9 @@ class RetrievalTrainingModule(torch.nn.Module):
         self._corpus_encoded = False
         self._searcher = None
         self._graphed = None                # captured corpus-encode forwards (mfar/modeling/graphed.py), kept across encodes
-        # precision of the CORPUS encode forwards: "fp32" | "fp16" | "bf16" (rows written to the slab are fp32 either way).  A module built
+        # precision of the CORPUS encode forwards: "fp32" | "fp16" | "bf16" | "int8" (rows written to the slab are fp32 either way).  A module built
         # directly encodes in fp32; the CLIs set it from their `precision` flag (commands/_setup.py `encode_precision_for`): the reference's
-        # default "16-mixed" (train.py:51) -> fp16 autocast.  MFAR_ENCODE_AUTOCAST=fp32|fp16|bf16 overrides either.
+        # default "16-mixed" (train.py:51) -> fp16 autocast.  MFAR_ENCODE_AUTOCAST=fp32|fp16|bf16|int8 overrides either.
         self.encode_precision = "fp32"
         # `hybrid_contrastive_loss_fn.bn.*` of a use_batchnorm run: trained by commands/train.py's loss object, unused at
         # evaluation (contrastive.py:685-694 applies no BatchNorm), carried through checkpoints under the reference's keys
@@ -219,14 +220,31 @@ class RetrievalTrainingModule(torch.nn.Module):
         max_len = int(self.encoder.get_max_seq_length())
         tb = os.environ.get("MFAR_ENCODE_TOKEN_BUDGET", "1")             # 0: always dev_batch_size texts; 1: the default; n > 1: n tokens
         budget = 0 if tb == "0" else (int(tb) if tb.isdigit() and int(tb) > 1 else bs * max_len)
-        # Precision of the corpus-encode forwards: `self.encode_precision`, overridden by MFAR_ENCODE_AUTOCAST=fp32|fp16|bf16.
+        # Precision of the corpus-encode forwards: `self.encode_precision`, overridden by MFAR_ENCODE_AUTOCAST=fp32|fp16|bf16|int8.
         # The reference encodes the corpus outside its precision plugin (which wraps the steps, not on_test_epoch_start) but with
         # torch.set_float32_matmul_precision("high") (train.py:67, mask_fields.py:52): fp32 matmuls may run with 10-bit-mantissa inputs on
         # its hardware.  gfx950 has no such fp32 mode; fp16 autocast IS that precision here (11-bit significand into fp32 accumulators):
         # measured on the BERT-base-shaped encoder, rows differ by 6e-4 of the largest value (bf16: 6e-3) at 3.1x the fp32 rate
         # (bench.py encode_pipeline).  The rows written to the slab are fp32 either way.
         mode = (os.environ.get("MFAR_ENCODE_AUTOCAST", "") or self.encode_precision or "fp32").lower()
-        ac = {"bf16": torch.bfloat16, "fp16": torch.float16}.get(mode)
+        # "int8": fp16 autocast with the transformer's linear layers in 8 bits, one scale per token and channel (mfar/modeling/quantized.py).
+        ac = {"bf16": torch.bfloat16, "fp16": torch.float16, "int8": torch.float16}.get(mode)
+        if mode == "int8" and dense:
+            from mfar.modeling.quantized import int8_linears
+            if self.device.type != "cuda":
+                raise ValueError("an int8 corpus encode needs the encoder on the GPU")
+            quantized = int8_linears(self.encoder[0])
+        else:
+            quantized = contextlib.nullcontext()
+        with quantized:
+            self._encode_dense(dense, prepare, bs, budget, max_len, ac)
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
+        _barrier()                                                               # :491 (no memmap reopen needed)
+        self._corpus_encoded = True
+
+    def _encode_dense(self, dense, prepare, bs, budget, max_len, ac) -> None:
+        """The forwards of on_eval_start: every dense field's distinct texts -> rows of the slab."""
         if dense and self._prefetch_backend() is not None:
             self._encode_fields_prefetched(dense, prepare, bs, budget, max_len, ac)
             dense = []                                       # (nothing left for the generic loop below)
@@ -276,10 +294,6 @@ class RetrievalTrainingModule(torch.nn.Module):
                 emb_u[torch.tensor(got, device=self.device)] = torch.stack(vecs).float()
             self._write_field(vec, docs, emb_u, torch.tensor([slot[t] for t in texts], device=self.device), bs)
             del emb_u
-        if self.device.type == "cuda":
-            torch.cuda.synchronize(self.device)
-        _barrier()                                                               # :491 (no memmap reopen needed)
-        self._corpus_encoded = True
 
     # -- the corpus encode with the host side off the critical path ---------------------------------------------------------------------
     # profiles/r05_p_encode_*: under bf16 autocast the GPU was busy 40 % of an encode; the rest was `PreTrainedTokenizerFast.__call__`'s

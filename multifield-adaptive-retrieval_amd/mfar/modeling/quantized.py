@@ -3,7 +3,8 @@
 One scale per token, computed on the fly, one per output channel, laid out once; exact integer sums on the matrix units at twice the rate of
 16-bit types.  There is no CPU form and no gradient: the layers serve forwards under `torch.no_grad()`.
 """
-from typing import Optional, Tuple
+import contextlib
+from typing import Iterator, Optional, Tuple
 
 import torch
 
@@ -40,9 +41,10 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return q, scale
 
 
-def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x [..., K] times 8-bit weights wq [N, K] with one scale per channel w_scale [N] (+ bias [N]) -> [..., N] of x's type, every token quantised
-    by its own scale on the way (`quantize_rows`); rounded once."""
+def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x [..., K] times 8-bit weights wq [N, K] with one scale per channel w_scale [N] (+ bias [N]) -> [..., N] of out_dtype (x's type if not
+    given), every token quantised by its own scale on the way (`quantize_rows`); rounded once."""
     dev = _native.op_device(x, wq, w_scale, bias)
     _check(x)
     K = x.shape[-1]
@@ -58,11 +60,46 @@ def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: 
     wq, w_scale = wq.contiguous(), w_scale.contiguous()
     if wq.data_ptr() % 16:
         wq = wq.clone()
-    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    y = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype or x.dtype, device=x.device)
     r = _rows(x)
     L = _native.lib()
     n = L.mfar_int8_linear_workspace_bytes(r.shape[0], K, N)
     work = torch.empty(n, dtype=torch.uint8, device=x.device)
     _native.check(L.mfar_int8_linear(dev, r.data_ptr(), _native.op_dtype(x), r.stride(0), r.shape[0], K, N, wq.data_ptr(), w_scale.data_ptr(),
-                                     None if bias is None else bias.data_ptr(), y.data_ptr(), work.data_ptr(), n, _native.op_stream(dev)))
+                                     None if bias is None else bias.data_ptr(), y.data_ptr(), _native.op_dtype(y), work.data_ptr(), n, _native.op_stream(dev)))
     return y
+
+
+class Int8Linear(torch.nn.Module):
+    """Inference form of a `torch.nn.Linear`: its weights as 8-bit rows (`weight`, `weight_scale`), its bias shared.  Under autocast the result has
+    autocast's type, as a Linear's has; the input is quantised from whatever type it arrives in."""
+
+    def __init__(self, linear: torch.nn.Linear):
+        super().__init__()
+        q, scale = quantize_rows(linear.weight.detach())
+        # (parameters, not buffers: what watches where an encoder's parameters live sees these too)
+        self.weight = torch.nn.Parameter(q, requires_grad=False)
+        self.weight_scale = torch.nn.Parameter(scale, requires_grad=False)
+        self.bias = linear.bias
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        out = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        return int8_linear(x, self.weight, self.weight_scale, self.bias, out_dtype=out)
+
+
+@contextlib.contextmanager
+def int8_linears(module: torch.nn.Module) -> Iterator[int]:
+    """While the context is open, every `torch.nn.Linear` below `module` is its `Int8Linear` (weights quantised as they are on entry); yields how
+    many.  For forwards under `torch.no_grad()`."""
+    swapped = []
+    try:
+        for parent in list(module.modules()):
+            for name, child in list(parent.named_children()):
+                if type(child) is torch.nn.Linear:
+                    swapped.append((parent, name, child))
+                    setattr(parent, name, Int8Linear(child))
+        yield len(swapped)
+    finally:
+        for parent, name, child in swapped:
+            setattr(parent, name, child)

@@ -31,8 +31,14 @@ class _Transformer(torch.nn.Module):
     def __init__(self, auto_model):
         super().__init__()
         self.auto_model = auto_model
+        self.fused_stack = ()        # (the T5 stack whose forward mfar/modeling/t5.py runs,); in a tuple: no second registration of its parameters
 
     def forward(self, features):
+        if self.fused_stack and features["input_ids"].is_cuda:
+            from mfar.modeling.t5 import attention_dropout, t5_encoder_forward
+            stack = self.fused_stack[0]
+            if not (stack.training and attention_dropout(stack) > 0):
+                return t5_encoder_forward(stack, features["input_ids"], features["attention_mask"])
         out = self.auto_model(input_ids=features["input_ids"], attention_mask=features["attention_mask"],
                               **({"token_type_ids": features["token_type_ids"]} if "token_type_ids" in features else {}))
         return out[0] if not hasattr(out, "last_hidden_state") else out.last_hidden_state
@@ -68,6 +74,13 @@ class SentenceEncoder(torch.nn.Sequential):
     @property
     def dense(self):
         return self._modules.get("2")
+
+    def use_fused_attention(self, enabled: bool = True) -> None:
+        """T5 encoders only (ValueError otherwise): forwards on the GPU go through the fused attention, forward and backward
+        (mfar/modeling/t5.py).  A training forward that drops attention weights (`dropout_rate` > 0 in train mode) stays with the stock attention:
+        the kernel has no dropout."""
+        from mfar.modeling.t5 import t5_stack
+        self[0].fused_stack = (t5_stack(self.auto_model),) if enabled else ()
 
     def get_sentence_embedding_dimension(self) -> int:
         if self.dense is not None:
