@@ -22,9 +22,11 @@
 #define AT_TILE 64        // keys (queries) staged in LDS per step
 #define AT_MAX_SAT 1023
 #define AT_MAX_STRIDE (1 << 22)
-// The running maximum of the softmax follows a tile's only when that is 2^8 over it: probabilities stay under 256 (fp16 holds them as exactly as
+// The running maximum of the softmax follows a tile's only when that is 2^8 over it: probabilities stay under 2^14 (fp16 holds them as exactly as
 // those under 1), and the accumulated output is hardly ever rescaled.
 #define AT_SLACK 8.0f
+// ... and the base lies 2^6 under the maximum it was set from, so that fp16 still holds what its rounding of a middling probability dropped (at_pack_lo).
+#define AT_SHIFT 6.0f
 
 // Waves per SIMD the register budget is set for.  From 2 on (256 registers) the compiler keeps accumulators where the vector unit reaches them;
 // with the whole file for one wave it parks them in accumulation registers and copies every score back and forth.
@@ -40,6 +42,7 @@ struct AttnParams {
     const int* start_ptr;        // [B] position of the first query among the keys, or NULL
     float *lse, *drow;           // [B, H, Lq], log2 units
     float* dpart;                // [blocks, H, n_buckets] partial bias gradients, or NULL
+    int* dexp;                   // [B, H, tiles of 128 queries] largest exponent of dO (fp16)
     int start, B, Lq, Lk, H, D, causal, n_buckets, n_side, sat;
     float scale;
     short first[129 * 2];        // first distance of each bucket of a side
@@ -73,8 +76,9 @@ template <typename T, int DP> __device__ __forceinline__ T* at_at(T* tile, int r
 
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
-// Steps of tiles held in LDS: two, so that one loads while the other is multiplied; one where two would leave a CU a single block.
-constexpr int at_stages(int size, int dp) { return size * dp >= 512 ? 1 : 2; }
+// Steps of tiles held in LDS: two, so that one loads while the other is multiplied; one where two would leave a CU a single block (the backward pass
+// holds more beside them).
+constexpr int at_stages(int size, int dp, bool backward) { return size * dp >= (backward ? 256 : 512) ? 1 : 2; }
 
 // Tiles of AT_TILE rows of one (batch, head) straight from memory to LDS: a wave's load instruction fills 1 KB in lane order, the swizzle of at_at is
 // applied on the addresses the lanes load from.  Rows >= n are not read (the last row stands in), nor are dims >= D (the row's first chunk stands in:
@@ -175,11 +179,12 @@ template <typename T> __device__ __forceinline__ V8<T> at_pack_lo(const f32x16& 
     return x;
 }
 // O' tiles of a wave (lane: one of 32 rows of the result, registers: dims) -> n rows of a [.., D] matrix `stride` elements apart, through LDS of the
-// wave's own (at_out_bytes), 64 dims at a time, so that a row leaves in runs of whole cache lines (8 bytes a lane of 32 rows
+// wave's own (at_out_bytes), 128 bytes of a row at a time, so that a row leaves in runs of whole cache lines (8 bytes a lane of 32 rows
 // straight from the registers: 83 us instead of 78 for the encode).
-template <typename T, int DP> constexpr int at_out_bytes() { return 32 * ((DP < 64 ? DP : 64) * (int)sizeof(T) + 16); }
+template <typename T, int DP> constexpr int at_out_dims() { return DP * (int)sizeof(T) < 128 ? DP : 128 / (int)sizeof(T); }
+template <typename T, int DP> constexpr int at_out_bytes() { return 32 * (at_out_dims<T, DP>() * (int)sizeof(T) + 16); }
 template <typename T, int DP> __device__ __forceinline__ void at_store(T* out, long long stride, int n, const f32x16* acc, float f, int D, void* lds) {
-    constexpr int W = DP < 64 ? DP : 64, PITCH = W * sizeof(T) + 16, LANES = W * sizeof(T) / 16, EACH = 16 / sizeof(T);
+    constexpr int W = at_out_dims<T, DP>(), PITCH = W * sizeof(T) + 16, LANES = W * sizeof(T) / 16, EACH = 16 / sizeof(T);
     const int l = threadIdx.x & 63, half = l >> 5;
     unsigned char* mine = (unsigned char*)lds;
 #pragma unroll
@@ -241,9 +246,9 @@ __device__ __forceinline__ void at_hide(f32x16& s, u32 seen) {
 
 // Runs `step(k0, bits, K, V)` for every tile of 64 keys in [0, end) that shows any key, with the tile's K and V in LDS; by the whole block.
 // tiles: at_stages of [K, V][AT_TILE][DP].  `ahead()` is run once, while the first tile is on its way.
-template <typename T, int DP, typename A, typename F>
+template <typename T, int DP, bool BACKWARD, typename A, typename F>
 __device__ __forceinline__ void at_for_tiles(const AttnParams& p, int b, int h, int end, T* tiles, A&& ahead, F&& step) {
-    constexpr int S = at_stages(sizeof(T), DP), SIZE = AT_TILE * DP;
+    constexpr int S = at_stages(sizeof(T), DP, BACKWARD), SIZE = AT_TILE * DP;
     const AtStream<T, DP> ks((const T*)p.k + b * p.k_b + h * p.k_h, p.k_l, end, p.D), vs((const T*)p.v + b * p.v_b + h * p.v_h, p.v_l, end, p.D);
     if (end <= 0) ahead();
     for (int base = 0; base < end; base += 64 * AT_TILE) {
@@ -333,9 +338,9 @@ __device__ __forceinline__ void at_softmax(f32x16 (&s)[N], T* vt, AtSoftmax& m, 
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
     top = max_halves(top);
     if (__any(top > m.limit)) {
-        const float up = top > m.limit ? top : 0.0f, keep = m.limit > 0.0f ? exp2_fast(-up) : 0.0f;   // (before the first key there is nothing to keep)
+        const float up = top > m.limit ? top - AT_SHIFT : 0.0f, keep = m.limit > 0.0f ? exp2_fast(-up) : 0.0f;   // (before the first key there is nothing to keep)
         m.base += up;
-        if (top > m.limit) m.limit = AT_SLACK;
+        if (top > m.limit) m.limit = AT_SHIFT + AT_SLACK;
         m.sum *= keep;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= keep;
@@ -379,7 +384,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     if (!at_place(p, (p.Lq + AT_COLS - 1) / AT_COLS, place)) return;
     extern __shared__ __align__(16) unsigned char at_lds[];
     T* tiles = (T*)at_lds;
-    float* lut = (float*)(tiles + at_stages(sizeof(T), DP) * 2 * AT_TILE * DP);
+    float* lut = (float*)(tiles + at_stages(sizeof(T), DP, false) * 2 * AT_TILE * DP);
     const int b = place.b, h = place.h, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5;
     const int start = at_start(p, b);
     const int q = place.tile * AT_COLS + wave * 32 + (l & 31);
@@ -395,7 +400,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     f32x16 acc[DP / 32] = {};
     AtSoftmax m;
     const float c = p.scale * LOG2E;
-    at_for_tiles<T, DP>(p, b, h, end, tiles, [&]() {
+    at_for_tiles<T, DP, false>(p, b, h, end, tiles, [&]() {
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) qf[s] = at_load<T>(qrow, live, s, p.D);
         at_lut(p, lut, h);
@@ -428,7 +433,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     if (p.lse && live && half == 0) p.lse[((long long)b * p.H + h) * p.Lq + q] = at_lse(m.base, sum);
 }
 
-// ---- forward, up to 32 queries (short texts, a decoder's next token): the work is in the keys ------------------------------------------------
+// ---- forward, few queries (short texts, a decoder's next token, small batches): the work of 32 queries is divided over the keys --------------------
 // Tiles of 32 keys go to the waves in turn, 4 waves a block and `splits` blocks per (batch, head): K straight into fragments, V through LDS of the
 // wave's own, no barrier in the loop, the next tile's loads in flight.  The waves' partial softmaxes are joined in LDS, the blocks' in a second
 // launch, both in a fixed order.  Bound by reading K and V.
@@ -449,11 +454,12 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     float* part = (float*)at_lds;                                          // [4 waves][DP][32], behind the loop
     float* stat = part + 4 * DP * 32;                                      // [4 waves][2][32]
     float* lut = stat + 4 * 64;
-    const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5, q = l & 31;
+    const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5, qi = l & 31;
+    const int q0 = (int)blockIdx.x / sp.splits * 32, part_of = (int)blockIdx.x % sp.splits, q = q0 + qi;
     const int start = at_start(p, b);
     const bool live = q < p.Lq;
     const int col = start + q;
-    const int end = p.causal ? min(p.Lk, max(start + p.Lq, 0)) : p.Lk;
+    const int end = p.causal ? min(p.Lk, max(start + min(p.Lq, q0 + 32), 0)) : p.Lk;
     constexpr int CH = DP / 8, NV = DP / 16;                               // chunks a row; chunks of V a lane
     const T* kb = (const T*)p.k + b * p.k_b + h * p.k_h;
     const T* vb = (const T*)p.v + b * p.v_b + h * p.v_h;
@@ -462,7 +468,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     V8<T> qf[DP / 16], kf[DP / 16], vr[NV];
     bool on = false;
     const int step = sp.splits * 4 * 32;
-    int k0 = ((int)blockIdx.x * 4 + wave) * 32;
+    int k0 = (part_of * 4 + wave) * 32;
     const bool vin = (l % CH) * 8 < p.D;
     auto fetch = [&]() {
         const int key = min(k0 + (l & 31), end - 1);
@@ -500,7 +506,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (seen) {
-            at_bias<1>(s[0], lut, p.sat, c, row0, col, start, p.causal != 0, run.base);
+            at_bias<1>(s[0], lut, p.sat, c, row0, col, start + q0, p.causal != 0, run.base);
             if (seen != ~0u) at_hide(s[0], seen);
             at_softmax<T, DP, KEEP, 1>(s, vt, run, acc);
         }
@@ -512,33 +518,33 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[(wave * DP + 32 * dt + crow(i, half)) * 32 + q] = acc[dt][i];
+        for (int i = 0; i < 16; ++i) part[(wave * DP + 32 * dt + crow(i, half)) * 32 + qi] = acc[dt][i];
     if (half == 0) {
-        stat[wave * 64 + q] = m;
-        stat[wave * 64 + 32 + q] = sum;
+        stat[wave * 64 + qi] = m;
+        stat[wave * 64 + 32 + qi] = sum;
     }
     __syncthreads();
     if (!live) return;
     float f[4], all = 0.0f;
-    m = fmaxf(fmaxf(stat[q], stat[64 + q]), fmaxf(stat[128 + q], stat[192 + q]));
+    m = fmaxf(fmaxf(stat[qi], stat[64 + qi]), fmaxf(stat[128 + qi], stat[192 + qi]));
     const float base = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        f[w] = exp2_fast(stat[w * 64 + q] - base);
-        all += f[w] * stat[w * 64 + 32 + q];
+        f[w] = exp2_fast(stat[w * 64 + qi] - base);
+        all += f[w] * stat[w * 64 + 32 + qi];
     }
     const long long row = ((long long)b * p.Lq + q) * p.H + h;
     const float norm = sp.splits == 1 ? at_norm(all) : 1.0f;
     for (int d = threadIdx.x >> 5; d < p.D; d += 8) {
         float x = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) x += f[w] * part[(w * DP + d) * 32 + q];
+        for (int w = 0; w < 4; ++w) x += f[w] * part[(w * DP + d) * 32 + qi];
         if (sp.splits == 1) at_write<T>(p, KEEP, row * p.D + d, x * norm);
-        else sp.o[(row * sp.splits + blockIdx.x) * p.D + d] = x;
+        else sp.o[(row * sp.splits + part_of) * p.D + d] = x;
     }
     if (threadIdx.x < 32) {
         if (sp.splits > 1) {
-            float* to = sp.ml + (row * sp.splits + blockIdx.x) * 2;
+            float* to = sp.ml + (row * sp.splits + part_of) * 2;
             to[0] = m, to[1] = all;
         } else if (p.lse) {
             p.lse[((long long)b * p.H + h) * p.Lq + q] = all == 0.0f ? -__builtin_inff() : m + __log2f(all);
@@ -573,30 +579,33 @@ template <typename T, bool KEEP> __global__ __launch_bounds__(AT_BLOCK) void mfa
     }
 }
 
-// Sums along the diagonals of a 32 x 32 tile (lanes: queries, registers: keys), added to sums[key - query]; by one wave, in memory of its own.
-// The tile goes through LDS: lane m of either half reads the 16 elements of its half's rows with (row - column) % 32 = m.  Those with row >= m lie on
-// diagonal m, the others on m - 32; half 0 then adds to the former, half 1 to the latter: 64 different places, no atomics (LDS float atomics
-// took 205 cycles per wave here, 16 of them per tile).
-__device__ __forceinline__ void at_diagonals(const f32x16& s, float* skew, float* sums) {
-    const int l = threadIdx.x & 63, half = l >> 5, m = l & 31;
+// Sums along the diagonals of a 32 x 32 tile (lanes: queries, registers: keys) times the lane's f, added to sums[key - query]; by one wave, in memory of
+// its own.  Element (key r, query q) goes to place r - q + 31 of row r of a 32 x 64 buffer: a diagonal is a column there, and what no element reaches
+// stays the zero it was set to once.  Every lane adds up a column and adds the sum to its distance's place: no atomics (LDS float atomics took 205
+// cycles a wave here, 16 of them a tile).
+#define AT_SKEW (32 * 64)
+__device__ __forceinline__ void at_diagonals(const f32x16& s, float f, float* skew, float* sums) {
+    const int l = threadIdx.x & 63, half = l >> 5, q = l & 31;
+    float* to = skew + 4 * half * 65 + 31 - q;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) skew[(crow(i, 0) + 4 * half) * 32 + m] = s[i];
+    for (int i = 0; i < 16; ++i) to[crow(i, 0) * 65] = s[i] * f;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    float all = 0.0f, on = 0.0f;
+    float t[2] = {};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const int r = 16 * half + j;
-        const float x = skew[r * 32 + ((r - m) & 31)];
-        all += x;
-        on += r >= m ? x : 0.0f;
-    }
-    const float off = sum_halves(all - on);
-    on = sum_halves(on);
-    sums[half ? m - 32 : m] += half ? off : on;
+    for (int r = 0; r < 32; ++r) t[r & 1] += skew[r * 64 + l];
+    if (l < 63) sums[l - 31] += t[0] + t[1];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
+
+// fp16 holds nothing under 2^-24: the score gradients dS are scaled by a power of two on their way into a product and back behind it, by each
+// query's own (dQ: queries in lanes) or by that of the (batch, head)'s largest dO (dK: summed over queries).  dP - D takes the factor in an fma.
+__device__ __forceinline__ int at_exponent(float largest) {
+    const int e = (int)((__float_as_uint(largest) >> 23) & 255) - 127;
+    return e > 100 ? 0 : max(e, -100);                                      // (infinities and NaN as they are)
+}
+__device__ __forceinline__ float at_pow2(int e) { return __uint_as_float((u32)(e + 127) << 23); }
 
 // ---- backward: dQ, the bias gradient, D ---------------------------------------------------------------------------------------------------
 template <typename T, int DP>
@@ -605,10 +614,11 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     if (!at_place(p, (p.Lq + AT_COLS - 1) / AT_COLS, place)) return;
     extern __shared__ __align__(16) unsigned char at_lds[];
     T* tiles = (T*)at_lds;
-    float* lut = (float*)(tiles + at_stages(sizeof(T), DP) * 2 * AT_TILE * DP);
+    float* lut = (float*)(tiles + at_stages(sizeof(T), DP, true) * 2 * AT_TILE * DP);
+    __shared__ int exps[4];
     const int n_lut = at_lut_size(p.sat);
     float* hist = lut + n_lut;                                             // [4 waves][n_lut] sums of dS by distance
-    float* skew = hist + 4 * n_lut;                                        // [4 waves][32][32]
+    float* skew = hist + 4 * n_lut;                                        // [4 waves][AT_SKEW]
     const int b = place.b, h = place.h, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5;
     const int start = at_start(p, b);
     const int q = place.tile * AT_COLS + wave * 32 + (l & 31);
@@ -620,11 +630,11 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const T* grow = (const T*)p.dout + b * p.do_b + (long long)q * p.do_l + h * p.do_h;
     const long long orow = (((long long)b * p.Lq + q) * p.H + h) * p.D, srow = ((long long)b * p.H + h) * p.Lq + q;
     V8<T> qf[DP / 16], gf[DP / 16];
-    float dsum = 0.0f, lse = 0.0f;
+    float dsum = 0.0f, lse = 0.0f, up = 1.0f, down = 1.0f;                 // up: the power of two dS is scaled by, down: back
     f32x16 acc[DP / 32] = {};
     float far_lo = 0.0f, far_hi = 0.0f;
     const float c = p.scale * LOG2E;
-    at_for_tiles<T, DP>(p, b, h, end, tiles, [&]() {
+    at_for_tiles<T, DP, true>(p, b, h, end, tiles, [&]() {
         if (live) lse = p.lse[srow];
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
@@ -636,10 +646,22 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
         }
         at_lut(p, lut, h);
         if (p.dpart)
-            for (int i = threadIdx.x; i < 4 * n_lut; i += AT_BLOCK) hist[i] = 0.0f;
+            for (int i = threadIdx.x; i < 4 * (n_lut + AT_SKEW); i += AT_BLOCK) hist[i] = 0.0f;
         dsum = sum_halves(dsum);
-        if (!live || lse == -__builtin_inff()) lse = __builtin_inff();      // no keys: P = exp2(-inf) = 0 everywhere
         if (live && half == 0) p.drow[srow] = dsum;
+        if (sizeof(T) == 2 && p.dexp) {
+            float largest = 0.0f;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) largest = fmaxf(largest, __builtin_fabsf((float)gf[s][j]));
+            int e = at_exponent(max_halves(largest));
+            up = at_pow2(-e), down = at_pow2(e);
+            for (int o = 1; o < 32; o <<= 1) e = max(e, __shfl_xor(e, o));
+            if (l == 0) exps[wave] = e;
+        }
+        if (!live || lse == -__builtin_inff()) lse = __builtin_inff();      // no keys: P = exp2(-inf) = 0 everywhere
+        dsum *= up;
     }, [&](int k0, u64 bits, T* kt, T* vt) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -654,7 +676,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
             const u32 shown = (u32)(bits >> (32 * t));
             if (shown != ~0u) at_hide(s, shown);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i]) * (dp[i] - dsum);
+            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i]) * __builtin_fmaf(dp[i], up, -dsum);
             if (p.dpart) {
                 if (row0 - col_lo - 31 >= p.sat) {
 #pragma unroll
@@ -663,7 +685,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
 #pragma unroll
                     for (int i = 0; i < 16; ++i) far_lo += s[i];
                 } else {
-                    at_diagonals(s, skew + wave * 1024, hist + wave * n_lut + (row0 - col_lo) + p.sat + AT_EDGE);
+                    at_diagonals(s, down, skew + wave * AT_SKEW, hist + wave * n_lut + (row0 - col_lo) + p.sat + AT_EDGE);
                 }
             }
 #pragma unroll
@@ -674,8 +696,10 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     });
     __syncthreads();                                                       // (the tiles' memory is free)
     const int q0 = place.tile * AT_COLS + wave * 32;
-    at_store<T, DP>((T*)p.dq + (((long long)b * p.Lq + q0) * p.H + h) * p.D, (long long)p.H * p.D, p.Lq - q0, acc, p.scale, p.D, at_lds + wave * at_out_bytes<T, DP>());
+    at_store<T, DP>((T*)p.dq + (((long long)b * p.Lq + q0) * p.H + h) * p.D, (long long)p.H * p.D, p.Lq - q0, acc, p.scale * down, p.D, at_lds + wave * at_out_bytes<T, DP>());
+    if (sizeof(T) == 2 && p.dexp && threadIdx.x == 0) p.dexp[((long long)b * p.H + h) * ((p.Lq + AT_COLS - 1) / AT_COLS) + place.tile] = max(max(exps[0], exps[1]), max(exps[2], exps[3]));
     if (p.dpart) {
+        far_lo *= down, far_hi *= down;
         for (int o = 1; o < 64; o <<= 1) {
             far_lo += __shfl_xor(far_lo, o);
             far_hi += __shfl_xor(far_hi, o);
@@ -726,7 +750,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     AtPlace place;
     if (!at_place(p, (p.Lk + AT_COLS - 1) / AT_COLS, place)) return;
     extern __shared__ __align__(16) unsigned char at_lds[];
-    constexpr int S = at_stages(sizeof(T), DP), SIZE = AT_TILE * DP;
+    constexpr int S = at_stages(sizeof(T), DP, true), SIZE = AT_TILE * DP;
     T* tiles = (T*)at_lds;                                                 // [S][Q, dO][AT_TILE][DP]
     float* stats = (float*)(tiles + S * 2 * SIZE);                          // [S][log2-sum, D][AT_TILE]
     float* lut = stats + S * 2 * AT_TILE;
@@ -745,14 +769,21 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     if (!__syncthreads_or(seen)) first = p.Lq;
     first = first / AT_TILE * AT_TILE;
     const AtStream<T, DP> qs(qb, p.q_l, p.Lq, p.D), gs(gb, p.do_l, p.Lq, p.D);
-    float mine = 0.0f;                                                     // thread i: entry i of the next tile's statistics
+    float mine = 0.0f, up = 1.0f, down = 1.0f;                              // thread i: entry i of the next tile's statistics
+    if (sizeof(T) == 2 && p.dexp) {
+        int e = -100;
+        const int n = (p.Lq + AT_COLS - 1) / AT_COLS;
+        for (int i = l; i < n; i += 64) e = max(e, p.dexp[((long long)b * p.H + h) * n + i]);
+        for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o));
+        up = at_pow2(-e), down = at_pow2(e);
+    }
     auto fetch = [&](int q0, int slot) {
         qs.load(q0, tiles + slot * 2 * SIZE);
         gs.load(q0, tiles + slot * 2 * SIZE + SIZE);
         if (threadIdx.x < 2 * AT_TILE) {
             const int i = threadIdx.x % AT_TILE;
             const bool in = q0 + i < p.Lq, d = threadIdx.x >= AT_TILE;
-            mine = in ? (d ? p.drow : p.lse)[srow + q0 + i] : 0.0f;
+            mine = in ? (d ? p.drow[srow + q0 + i] * up : p.lse[srow + q0 + i]) : 0.0f;
             // rows behind the last and rows that saw nothing: P = exp2(s - inf) = 0
             if (!d && (!in || mine == -__builtin_inff())) mine = __builtin_inff();
             stats[slot * 2 * AT_TILE + threadIdx.x] = mine;
@@ -793,7 +824,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
             for (int i = 0; i < 16; ++i) {
                 const int r = 32 * t + crow(i, half);
                 s[i] = exp2_fast(s[i] - rows[r]);
-                dp[i] = s[i] * (dp[i] - rows[AT_TILE + r]);
+                dp[i] = s[i] * __builtin_fmaf(dp[i], up, -rows[AT_TILE + r]);
             }
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
@@ -816,6 +847,6 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const int k0 = key0 + wave * 32;
     const long long at = (((long long)b * p.Lk + k0) * p.H + h) * p.D;
     void* lds = at_lds + wave * at_out_bytes<T, DP>();
-    at_store<T, DP>((T*)p.dk + at, (long long)p.H * p.D, p.Lk - k0, dk, p.scale, p.D, lds);
+    at_store<T, DP>((T*)p.dk + at, (long long)p.H * p.D, p.Lk - k0, dk, p.scale * down, p.D, lds);
     at_store<T, DP>((T*)p.dv + at, (long long)p.H * p.D, p.Lk - k0, dv, 1.0f, p.D, lds);
 }

@@ -55,30 +55,10 @@ template <typename T> __device__ __forceinline__ u64 q8_pack(const V8<T>& x, flo
     return w;
 }
 
-// Rows of x -> 8-bit rows (ldq bytes apart; pad: bytes [K, ldq) become zeros) and their scales.  One wave per row; a row is read once while it fits
-// the registers.  Bound by reading x: 32768 x 768 fp16 (75 MB) 16 us.
-// The blocks behind the rows' copy weights (launch count: one).
-template <typename T>
-__global__ __launch_bounds__(256) void mfar_quantize_rows_kernel(const T* x, long long ldx, int M, int K, signed char* q, long long ldq, float* scale, int pad, const Int8Copy cp) {
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, row = blockIdx.x * 4 + wave;
-    const int row_blocks = (M + 3) / 4;
-    if ((int)blockIdx.x >= row_blocks) {
-        for (int r = ((int)blockIdx.x - row_blocks) * 4 + wave; r < cp.rows; r += ((int)gridDim.x - row_blocks) * 4) {
-            const signed char* from = cp.from + (long long)r * cp.n;
-            for (int k = l * 8; k < cp.n; k += 512) {
-                u64 w = 0;
-                if (k + 8 <= cp.n) __builtin_memcpy(&w, from + k, 8);
-                else
-                    for (int j = 0; k + j < cp.n; ++j) w |= (u64)(unsigned char)from[k + j] << (8 * j);
-                *(u64*)(cp.to + (long long)r * cp.ld + k) = w;
-            }
-        }
-        return;
-    }
-    if (row >= M) return;
-    const T* xr = x + (long long)row * ldx;
-    signed char* qr = q + (long long)row * ldq;
-    const int chunks = (K + 7) / 8;
+// One row by one wave: K elements of xr -> bytes at qr, of which [K, ldq) become zeros with pad; returns the scale.  The row is read once while it fits
+// the registers.
+template <typename T> __device__ __forceinline__ float q8_row(const T* xr, int K, signed char* qr, long long ldq, bool pad) {
+    const int l = threadIdx.x & 63, chunks = (K + 7) / 8;
     V8<T> kept[Q8_KEPT];
     float top = 0.0f;
 #pragma unroll
@@ -100,7 +80,6 @@ __global__ __launch_bounds__(256) void mfar_quantize_rows_kernel(const T* x, lon
     }
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const float s = top == __builtin_inff() ? __builtin_nanf("") : top / 127.0f;
-    if (l == 0) scale[row] = s;
     const bool live = s > 0.0f, quick = s > 1e-30f && (__float_as_uint(s) & 0x7fffff) != 0x7fffff;
     const float y = 1.0f / s;
     auto put = [&](int c, const V8<T>& v) {
@@ -115,6 +94,32 @@ __global__ __launch_bounds__(256) void mfar_quantize_rows_kernel(const T* x, lon
     for (int c = Q8_KEPT * 64 + l; c < chunks; c += 64) put(c, q8_load<T>(xr, c, K));
     if (pad)
         for (long long c = chunks + l; c < ldq / 8; c += 64) *(u64*)(qr + 8 * c) = 0;
+    return s;
+}
+
+// Rows of x -> 8-bit rows (ldq bytes apart; pad: bytes [K, ldq) become zeros) and their scales.  One wave per row.
+// Bound by reading x: 32768 x 768 fp16 (75 MB) 20 us, 16384 x 4096 bf16 (201 MB) 46 us.
+// The blocks behind the rows' copy weights (launch count: one).
+template <typename T>
+__global__ __launch_bounds__(256) void mfar_quantize_rows_kernel(const T* x, long long ldx, int M, int K, signed char* q, long long ldq, float* scale, int pad, const Int8Copy cp) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, row = blockIdx.x * 4 + wave;
+    const int row_blocks = (M + 3) / 4;
+    if ((int)blockIdx.x >= row_blocks) {
+        for (int r = ((int)blockIdx.x - row_blocks) * 4 + wave; r < cp.rows; r += ((int)gridDim.x - row_blocks) * 4) {
+            const signed char* from = cp.from + (long long)r * cp.n;
+            for (int k = l * 8; k < cp.n; k += 512) {
+                u64 w = 0;
+                if (k + 8 <= cp.n) __builtin_memcpy(&w, from + k, 8);
+                else
+                    for (int j = 0; k + j < cp.n; ++j) w |= (u64)(unsigned char)from[k + j] << (8 * j);
+                *(u64*)(cp.to + (long long)r * cp.ld + k) = w;
+            }
+        }
+        return;
+    }
+    if (row >= M) return;
+    const float s = q8_row<T>(x + (long long)row * ldx, K, q + (long long)row * ldq, ldq, pad != 0);
+    if (l == 0) scale[row] = s;
 }
 
 struct Int8Params {
@@ -149,6 +154,72 @@ template <typename T> __device__ __forceinline__ void q8_store(const Int8Params&
     }
 }
 
+// 16 bytes of a channel's weights.  Past a row's end they may be anything (x holds zeros there), but past the last row's end nothing is read.
+__device__ __forceinline__ i32x4 q8_weights(const Int8Params& p, int n, int k) {
+    i32x4 w = {};
+    if (k < p.K) {
+        const long long at = (long long)min(n, p.N - 1) * p.ldw + k, end = (long long)(p.N - 1) * p.ldw + p.K;
+        if (at + 16 <= end) {
+            __builtin_memcpy(&w, p.wq + at, 16);
+        } else {
+            signed char tail[16];
+            for (int j = 0; j < 16; ++j) tail[j] = at + j < end ? p.wq[at + j] : (signed char)0;
+            __builtin_memcpy(&w, tail, 16);
+        }
+    }
+    return w;
+}
+
+// ---- up to 32 tokens: quantising and product in one launch ------------------------------------------------------------------------------------
+// Every block quantises all rows into LDS (they are few) while its first weights are on their way, then multiplies 32 channels by them, k divided over
+// the waves.  12 x 768 x 768: one launch of 6 us for two of 9.
+#define Q8_FEW_ROWS 32
+#define Q8_FEW_K 2048
+template <typename T, typename X>
+__global__ __launch_bounds__(256) void mfar_int8_few_kernel(const Int8Params p, const X* x, long long ldx) {
+    extern __shared__ __align__(16) signed char q8_lds[];                  // [32][Kp + 16] rows, then partial sums
+    __shared__ float scales[Q8_FEW_ROWS];
+    const int n0 = blockIdx.x * 32, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, half = l >> 5;
+    const int pitch = p.Kp + 16;
+    i32x4 a[4];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) a[u] = q8_weights(p, n0 + (l & 31), k0 + u * 128 + 16 * half);
+    };
+    fetch(wave * 32);
+    for (int r = wave; r < p.M; r += 4) {
+        const float s = q8_row<X>(x + (long long)r * ldx, p.K, q8_lds + r * pitch, p.Kp, true);
+        if (l == 0) scales[r] = s;
+    }
+    __syncthreads();
+    const signed char* row = q8_lds + min(l & 31, p.M - 1) * pitch + 16 * half;
+    i32x16 acc = {};
+    for (int k0 = wave * 32; k0 < p.K; k0 += 4 * 128) {
+        i32x4 b[4], now[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            now[u] = a[u];
+            b[u] = k0 + u * 128 + 16 * half < p.Kp ? *(const i32x4*)(row + k0 + u * 128) : i32x4{};
+        }
+        if (k0 + 4 * 128 < p.K) fetch(k0 + 4 * 128);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(now[u], b[u], acc, 0, 0, 0);
+    }
+    __syncthreads();                                                       // (the rows' memory takes the partial sums)
+    int* part = (int*)q8_lds;                                              // [3][64][17]
+    if (wave) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[((wave - 1) * 64 + l) * 17 + i] = acc[i];
+    }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] += part[l * 17 + i] + part[(64 + l) * 17 + i] + part[(128 + l) * 17 + i];
+    Int8Params o = p;
+    o.xs = scales;
+    q8_store<T>(o, acc, n0, l & 31);
+}
+
 // ---- few tiles: one 32 x 32 tile per block, its k divided over the 4 waves, fragments straight from memory -------------------------------------
 // Bound by latency: every load of a wave's share is in flight at once.  Rows of the weights may start anywhere.
 template <typename T>
@@ -156,29 +227,13 @@ __global__ __launch_bounds__(256) void mfar_int8_tile_kernel(const Int8Params p)
     __shared__ int part[3][64][17];
     const int n0 = blockIdx.x * 32, m0 = blockIdx.y * 32, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, half = l >> 5;
     const signed char* x = p.xq + (long long)min(m0 + (l & 31), p.M - 1) * p.ldx;
-    const long long w0 = (long long)min(n0 + (l & 31), p.N - 1) * p.ldw, w_end = (long long)(p.N - 1) * p.ldw + p.K;
     i32x16 acc = {};
-    auto weights = [&](int k) {
-        // past a row's end the weights may be anything (x holds zeros there), but past the last row's end nothing is read
-        i32x4 w = {};
-        if (k < p.K) {
-            const long long at = w0 + k;
-            if (at + 16 <= w_end) {
-                __builtin_memcpy(&w, p.wq + at, 16);
-            } else {
-                signed char tail[16];
-                for (int j = 0; j < 16; ++j) tail[j] = at + j < w_end ? p.wq[at + j] : (signed char)0;
-                __builtin_memcpy(&w, tail, 16);
-            }
-        }
-        return w;
-    };
     for (int k0 = wave * 32; k0 < p.K; k0 += 4 * 128) {
         i32x4 a[4], b[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int k = k0 + u * 128 + 16 * half;
-            a[u] = weights(k);
+            a[u] = q8_weights(p, n0 + (l & 31), k);
             b[u] = k < p.Kp ? *(const i32x4*)(x + k) : i32x4{};
         }
 #pragma unroll

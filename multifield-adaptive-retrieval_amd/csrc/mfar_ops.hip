@@ -123,25 +123,26 @@ AttnParams attention_params(const mfar_attention* a) {
 }
 int64_t drow_bytes(const mfar_attention* a) { return ((int64_t)a->B * a->H * a->Lq * 4 + 15) / 16 * 16; }
 // (behind the loop the tiles' memory takes the results on their way out)
-template <typename T, int DP> constexpr size_t tile_bytes() {
-    constexpr size_t n = at_stages(sizeof(T), DP) * 2ull * AT_TILE * DP * sizeof(T);
-    static_assert(n >= 4 * at_out_bytes<T, DP>());
+template <typename T, int DP> constexpr size_t tile_bytes(bool backward) {
+    const size_t n = at_stages(sizeof(T), DP, backward) * 2ull * AT_TILE * DP * sizeof(T);
+    static_assert(at_stages(sizeof(T), DP, true) * 2ull * AT_TILE * DP * sizeof(T) >= 4 * at_out_bytes<T, DP>());
     return n;
 }
+int64_t dexp_bytes(const mfar_attention* a) { return a->dtype == MFAR_DTYPE_F16 ? ((int64_t)a->B * a->H * cdiv(a->Lq, AT_COLS) * 4 + 15) / 16 * 16 : 0; }
 size_t lut_bytes(const AttnParams& p) { return (size_t)(2 * (p.sat + AT_EDGE) + 1) * 4; }
 
-// Up to 32 queries take the kernel that divides the keys over waves and blocks; a block gets at least 8 tiles of 32 keys, and there are no more
-// blocks than about four per CU.
-bool few_queries(const mfar_attention* a) { return a->Lq <= 32; }
+// Up to 32 queries, and batches of fewer than 256 blocks of 128 (one per CU), take the kernel that divides the keys over waves and blocks
+// (7 x 4 heads x 213 fp32: 25 us as 56 blocks); a block gets at least 8 tiles of 32 keys, and there are no more blocks than about four per CU.
+bool few_queries(const mfar_attention* a) { return a->Lq <= 32 || cdiv(a->Lq, AT_COLS) * a->B * a->H < 256; }
 int key_splits(const mfar_attention* a) {
-    return (int)std::max<int64_t>(1, std::min(cdiv(1024, (int64_t)a->B * a->H), cdiv(a->Lk, 8 * 32)));
+    return (int)std::max<int64_t>(1, std::min(cdiv(1024, cdiv(a->Lq, 32) * a->B * a->H), cdiv(a->Lk, 8 * 32)));
 }
 int64_t split_rows(const mfar_attention* a) { return (int64_t)a->B * a->Lq * a->H * key_splits(a); }
 int64_t split_bytes(const mfar_attention* a) { return few_queries(a) && key_splits(a) > 1 ? split_rows(a) * (a->D + 2) * 4 : 0; }
 
 template <typename T, int DP, bool KEEP> int attention_few(const AttnParams& p, const AttnSplit& sp, hipStream_t st) {
     const size_t lds = 4ull * DP * 32 * 4 + 4 * 64 * 4 + lut_bytes(p);     // (the V tiles, 4 * 32 * DP elements, lie in its first part)
-    int rc = launch<mfar_attn_few_kernel<T, DP, KEEP>>("mfar_attn_few_kernel", dim3(sp.splits, p.H, p.B), lds, st, p, sp);
+    int rc = launch<mfar_attn_few_kernel<T, DP, KEEP>>("mfar_attn_few_kernel", dim3(cdiv(p.Lq, 32) * sp.splits, p.H, p.B), lds, st, p, sp);
     if (rc == MFAR_OK && sp.splits > 1)
         rc = launch<mfar_attn_join_kernel<T, KEEP>>("mfar_attn_join_kernel", dim3(cdiv((int64_t)p.B * p.Lq * p.H, 4)), 0, st, p, sp);
     return rc;
@@ -155,17 +156,17 @@ template <typename T, int DP> int attention_forward(const AttnParams& p, const A
             if (p.out_lo) return attention_few<T, DP, true>(p, sp, st);
         return attention_few<T, DP, false>(p, sp, st);
     }
-    const size_t lds = tile_bytes<T, DP>() + lut_bytes(p);
+    const size_t lds = tile_bytes<T, DP>(false) + lut_bytes(p);
     const dim3 grid(at_grid(p, p.Lq));
     if constexpr (sizeof(T) == 2)
         if (p.out_lo) return launch<mfar_attn_forward_kernel<T, DP, true>>("mfar_attn_forward_kernel", grid, lds, st, p);
     return launch<mfar_attn_forward_kernel<T, DP, false>>("mfar_attn_forward_kernel", grid, lds, st, p);
 }
 template <typename T, int DP> int attention_backward(const AttnParams& p, float* dtable, hipStream_t st) {
-    constexpr int S = at_stages(sizeof(T), DP);
-    const size_t tiles = tile_bytes<T, DP>();
+    constexpr int S = at_stages(sizeof(T), DP, true);
+    const size_t tiles = tile_bytes<T, DP>(true);
     const dim3 grid(at_grid(p, p.Lq));
-    int rc = launch<mfar_attn_dq_kernel<T, DP>>("mfar_attn_dq_kernel", grid, tiles + lut_bytes(p) * (p.dpart ? 5 : 1) + (p.dpart ? 4 * 1024 * 4 : 0), st, p);
+    int rc = launch<mfar_attn_dq_kernel<T, DP>>("mfar_attn_dq_kernel", grid, tiles + lut_bytes(p) * (p.dpart ? 5 : 1) + (p.dpart ? 4 * AT_SKEW * 4 : 0), st, p);
     if (rc != MFAR_OK) return rc;
     if (p.Lk) {
         rc = launch<mfar_attn_dkv_kernel<T, DP>>("mfar_attn_dkv_kernel", dim3(at_grid(p, p.Lk)), tiles + S * 2 * AT_TILE * 4 + lut_bytes(p), st, p);
@@ -236,6 +237,13 @@ template <typename T> int int8_product(const Int8Params& p, hipStream_t st) {
     if (cdiv(p.M, 256) * cdiv(p.N, 256) >= 256) return int8_gemm<T, 2, 4, 4, 2>(p, st);
     return int8_gemm<T, 2, 2, 2, 2>(p, st);
 }
+template <typename T, typename X> int int8_few(const Int8Params& p, const void* x, int64_t ldx, hipStream_t st) {
+    const size_t lds = std::max<size_t>(Q8_FEW_ROWS * (size_t)(p.Kp + 16), 3 * 64 * 17 * 4);
+    return launch<mfar_int8_few_kernel<T, X>>("mfar_int8_few_kernel", dim3(cdiv(p.N, 32)), lds, st, p, (const X*)x, (long long)ldx);
+}
+template <typename T> int int8_few_f32(const Int8Params& p, const void* x, int64_t ldx, hipStream_t st) { return int8_few<T, float>(p, x, ldx, st); }
+template <typename T> int int8_few_bf16(const Int8Params& p, const void* x, int64_t ldx, hipStream_t st) { return int8_few<T, __bf16>(p, x, ldx, st); }
+template <typename T> int int8_few_f16(const Int8Params& p, const void* x, int64_t ldx, hipStream_t st) { return int8_few<T, _Float16>(p, x, ldx, st); }
 int check_rows(const void* x, int dtype, int64_t ldx, int64_t M, int K) {
     if (!type_size(dtype)) return bad("dtype must be F32, BF16 or F16");
     if (M < 0 || M > (1 << 23) || K < 1 || K > Q8_MAX_K) return bad("M must be 0..2^23, K 1..131072");
@@ -244,6 +252,8 @@ int check_rows(const void* x, int dtype, int64_t ldx, int64_t M, int K) {
     return MFAR_OK;
 }
 int64_t padded_k(int K) { return cdiv(K, Q8_STEP) * Q8_STEP; }
+// Few enough rows for every block to quantise them all.
+bool few_rows(int64_t M, int K) { return M <= Q8_FEW_ROWS && K <= Q8_FEW_K; }
 bool copies_weights(int64_t M, int64_t N, int K) { return K % 16 && !small_product(M, N); }   // rows have to start on 16 bytes
 int64_t int8_scales_at(int64_t M, int K) { return M * padded_k(K); }
 int64_t int8_weights_at(int64_t M, int K) { return int8_scales_at(M, K) + cdiv(M * 4, 16) * 16; }
@@ -255,7 +265,7 @@ extern "C" int64_t mfar_attention_workspace_bytes(const mfar_attention* a, int b
     if (rc != MFAR_OK) return rc;
     if (a->B == 0 || a->Lq == 0) return 0;
     if (!backward) return split_bytes(a);
-    return drow_bytes(a) + (a->dtable ? cdiv(a->Lq, AT_COLS) * a->B * a->H * a->n_buckets * 4 : 0);
+    return drow_bytes(a) + dexp_bytes(a) + (a->dtable ? cdiv(a->Lq, AT_COLS) * a->B * a->H * a->n_buckets * 4 : 0);
 }
 extern "C" int mfar_attention_forward(int device, const mfar_attention* a, void* stream) {
     int rc = check_attention(a, false);
@@ -275,7 +285,8 @@ extern "C" int mfar_attention_backward(int device, const mfar_attention* a, void
     ON_DEVICE(device);
     AttnParams p = attention_params(a);
     p.drow = (float*)a->workspace;
-    p.dpart = a->dtable ? (float*)((char*)a->workspace + drow_bytes(a)) : nullptr;
+    p.dexp = a->dtype == MFAR_DTYPE_F16 ? (int*)((char*)a->workspace + drow_bytes(a)) : nullptr;
+    p.dpart = a->dtable ? (float*)((char*)a->workspace + drow_bytes(a) + dexp_bytes(a)) : nullptr;
     return FOR_TYPE_AND_DIM(attention_backward, p, a->dtable, (hipStream_t)stream);
 }
 
@@ -289,6 +300,7 @@ extern "C" int mfar_quantize_rows(int device, const void* x, int dtype, int64_t 
 }
 extern "C" int64_t mfar_int8_linear_workspace_bytes(int64_t M, int K, int N) {
     if (M < 0 || K < 1 || N < 0) return bad("M and N must be >= 0, K >= 1");
+    if (few_rows(M, K)) return 0;
     return int8_weights_at(M, K) + (copies_weights(M, N, K) ? (int64_t)N * padded_k(K) : 0);
 }
 extern "C" int mfar_int8_linear(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int N, const int8_t* wq, const float* w_scale,
@@ -300,12 +312,19 @@ extern "C" int mfar_int8_linear(int device, const void* x, int dtype, int64_t ld
     if (M == 0 || N == 0) return MFAR_OK;
     if (!wq || !w_scale || !y) return bad("NULL tensor");
     if (!aligned16(wq)) return bad("the weights must be 16-byte aligned");
+    hipStream_t st = (hipStream_t)stream;
+    if (few_rows(M, K)) {
+        ON_DEVICE(device);
+        const Int8Params p = {nullptr, (const signed char*)wq, nullptr, w_scale, bias, y, 0, (long long)K, false, (int)M, N, K, (int)padded_k(K)};
+        return dtype == MFAR_DTYPE_F32    ? FOR_TYPE(y_dtype, int8_few_f32, p, x, ldx, st)
+               : dtype == MFAR_DTYPE_BF16 ? FOR_TYPE(y_dtype, int8_few_bf16, p, x, ldx, st)
+                                          : FOR_TYPE(y_dtype, int8_few_f16, p, x, ldx, st);
+    }
     if (!workspace || !aligned16(workspace) || workspace_bytes < mfar_int8_linear_workspace_bytes(M, K, N)) return bad("workspace too small or not 16-byte aligned");
     ON_DEVICE(device);
     const int64_t Kp = padded_k(K);
     int8_t* xq = (int8_t*)workspace;
     float* xs = (float*)((char*)workspace + int8_scales_at(M, K));
-    hipStream_t st = (hipStream_t)stream;
     Int8Copy cp = {};
     const signed char* w = (const signed char*)wq;
     int64_t ldw = K;

@@ -64,9 +64,9 @@ def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: 
     r = _rows(x)
     L = _native.lib()
     n = L.mfar_int8_linear_workspace_bytes(r.shape[0], K, N)
-    work = torch.empty(n, dtype=torch.uint8, device=x.device)
+    work = torch.empty(n, dtype=torch.uint8, device=x.device) if n > 0 else None
     _native.check(L.mfar_int8_linear(dev, r.data_ptr(), _native.op_dtype(x), r.stride(0), r.shape[0], K, N, wq.data_ptr(), w_scale.data_ptr(),
-                                     None if bias is None else bias.data_ptr(), y.data_ptr(), _native.op_dtype(y), work.data_ptr(), n, _native.op_stream(dev)))
+                                     None if bias is None else bias.data_ptr(), y.data_ptr(), _native.op_dtype(y), None if work is None else work.data_ptr(), n, _native.op_stream(dev)))
     return y
 
 

@@ -179,6 +179,24 @@ def test_attention_gradients_against_differences():
         assert abs(quotient - along) < 1e-3 * size, (i, quotient, along, size)
 
 
+@pytest.mark.parametrize("size", [2.0 ** -10, 2.0 ** 8])
+def test_attention_gradients_of_small_and_large_losses(size):
+    """A power of two on dout is a power of two on every gradient, fp16's own rounding apart: the score gradients of a small loss do not drown in fp16's
+    smallest numbers, those of a large one do not overflow on the way.  (2^-10: dS near 2^-17, of which fp16 by itself would keep 7 bits.)"""
+    q, k, v, table, dout = _attention_inputs(15, 2, 150, 150, 2, 64, "fp16")
+    dout = (dout.float().clamp(-4, 4) * 0.25).half()
+    dout = torch.where(dout.abs() < 2.0 ** -4, dout.sign() * 2.0 ** -4, dout)          # exact after scaling: no subnormal numbers in dout itself
+    one = _run_attention(q, k, v, table, (dout.float() * 2.0 ** -2).half())
+    got = _run_attention(q, k, v, table, (dout.float() * size).half())
+    f = size * 4
+    assert torch.equal(got["dtable"], one["dtable"] * f)
+    for n in ("dq", "dk", "dv"):
+        a, b = got[n].double() / f, one[n].double()
+        # one rounding each; what lies in fp16's smallest numbers is off by half their step
+        tol = 2.0 ** -11 * (a.abs() + b.abs()) + 2.0 ** -25 / f + 2.0 ** -25
+        assert bool(((a - b).abs() <= tol).all()), n
+
+
 def test_attention_is_reproducible_and_follows_the_current_stream():
     q, k, v, table, dout = _attention_inputs(10, 3, 300, 300, 4, 64, "bf16")
     a = _run_attention(q, k, v, table, dout)
@@ -290,13 +308,26 @@ def _int8_check(x, wq, ws, b, got):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
-@pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 768, 768), (12, 768, 769), (33, 64, 96), (129, 1001, 519), (300, 130, 257), (1000, 1536, 768), (70, 4096, 33),
+@pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 768, 768), (12, 768, 769), (32, 2048, 65), (31, 2000, 100), (32, 2049, 40), (33, 64, 96), (129, 1001, 519), (300, 130, 257), (1000, 1536, 768), (70, 4096, 33),
                                    (513, 17, 1030), (3000, 200, 1500), (2049, 1000, 1025), (1700, 136, 1700), (4100, 144, 4200), (4000, 300, 4097)])
 def test_int8_linear(dtype, M, K, N):
     from mfar.modeling.quantized import int8_linear
     print(f"int8 {dtype} {M} {K} {N}", flush=True)
     x, wq, ws, b = _int8_case(M, K, N, dtype, (M + N) % 2 == 0)
     _int8_check(x, wq, ws, b, int8_linear(x, wq, ws, b))
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_int8_linear_result_types(M):
+    from mfar.modeling.quantized import int8_linear
+    x, wq, ws, b = _int8_case(M, 130, 72, "fp16", True)
+    exact = int8_linear(x, wq, ws, b, out_dtype=torch.float32)
+    for t in (torch.float16, torch.bfloat16, torch.float32):
+        got = int8_linear(x, wq, ws, b, out_dtype=t)
+        assert got.dtype == t and torch.equal(got, exact.to(t))
+        assert torch.equal(int8_linear(x.float(), wq, ws, b, out_dtype=t), got)
+    with pytest.raises(TypeError):
+        int8_linear(x, wq, ws, b, out_dtype=torch.float64)
 
 
 def test_int8_linear_layouts_extremes_and_poison():

@@ -79,9 +79,9 @@ def test_int8_and_distillation_refusals_at_the_c_abi():
     assert L.mfar_quantize_rows(0, P, F16, -64, 4, 64, P, 64, P, None) == -1
     assert L.mfar_quantize_rows(0, None, F16, 64, 4, 64, P, 64, P, None) == -1
     assert L.mfar_quantize_rows(0, None, F16, 64, 0, 64, None, 64, None, None) == 0
-    n = L.mfar_int8_linear_workspace_bytes(10, 100, 20)
-    assert n >= 10 * 100 + 10 * 4 and L.mfar_int8_linear_workspace_bytes(-1, 5, 5) == -1
-    ok = [0, P, F16, 100, 10, 100, 20, P, P, None, P, F16, P, n, None]
+    n = L.mfar_int8_linear_workspace_bytes(40, 100, 20)
+    assert n >= 40 * 100 + 40 * 4 and L.mfar_int8_linear_workspace_bytes(10, 100, 20) == 0 and L.mfar_int8_linear_workspace_bytes(-1, 5, 5) == -1
+    ok = [0, P, F16, 100, 40, 100, 20, P, P, None, P, F16, P, n, None]
     for i, v in ((2, 5), (3, -1), (4, -1), (5, 0), (6, -1), (6, 2 ** 23 + 1), (7, None), (7, P + 4), (8, None), (10, None), (11, 4), (12, None), (12, P + 8), (13, n - 1)):
         args = list(ok)
         args[i] = v
