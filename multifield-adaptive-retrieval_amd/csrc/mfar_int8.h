@@ -25,12 +25,18 @@ struct Int8Copy {
     int rows, n;
 };
 
-template <typename T> __device__ __forceinline__ V8<T> q8_load(const T* row, int c, int K) {
+// chunk c (8 elements) of a row that may start anywhere: an unaligned vector load
+template <typename T> __device__ __forceinline__ V8<T> q8_load(const T* row, int c) {
+    V8<T> x;
+    __builtin_memcpy(&x, row + 8 * c, sizeof x);
+    return x;
+}
+// the chunk that the row's end cuts, zeros behind it
+template <typename T> __device__ __forceinline__ V8<T> q8_load_cut(const T* row, int c, int K) {
     V8<T> x = {};
-    if (8 * c + 8 <= K) __builtin_memcpy(&x, row + 8 * c, sizeof x);       // (rows may start anywhere: unaligned vector loads)
-    else
-        for (int j = 0; j < 8; ++j)
-            if (8 * c + j < K) x[j] = row[8 * c + j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (8 * c + j < K) x[j] = row[8 * c + j];
     return x;
 }
 // |x| with NaN as infinity, so that a maximum keeps it
@@ -38,63 +44,83 @@ __device__ __forceinline__ float q8_size(float x) {
     const float a = __builtin_fabsf(x);
     return a <= 3.4028234e38f ? a : __builtin_inff();
 }
-// rint(x / s) as a byte, the quotient rounded to fp32 first.  quick: y = 1 / s rounded, then one step of the remainder gives the correctly rounded
-// quotient (Markstein; not for divisors of an all-ones mantissa, nor where 1 / s or the remainder would leave the normal range); adding 1.5 * 2^23
-// leaves the whole number in the low byte.
-__device__ __forceinline__ u32 q8_byte(float x, float s, float y, bool quick) {
-    if (quick) {
-        const float q = x * y;
-        return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, s, x), y, q) + 12582912.0f) & 0xffu;
+// A row's scale and the bytes under it: rint(x / s), the quotient rounded to fp32 first.  quick: y = 1 / s rounded, then one step of the remainder gives
+// the correctly rounded quotient (Markstein; not for divisors of an all-ones mantissa, nor where 1 / s or the remainder would leave the normal
+// range); adding 1.5 * 2^23 leaves the whole number in the low byte.
+struct Q8Divisor {
+    float s, y;
+    bool live, quick;
+    __device__ __forceinline__ explicit Q8Divisor(float top) {
+        s = top == __builtin_inff() ? __builtin_nanf("") : top / 127.0f;
+        live = s > 0.0f;
+        quick = s > 1e-30f && (__float_as_uint(s) & 0x7fffff) != 0x7fffff;
+        y = 1.0f / s;
     }
-    return (u32)(int)fminf(fmaxf(__builtin_rintf(x / s), -127.0f), 127.0f) & 0xffu;
-}
-template <typename T> __device__ __forceinline__ u64 q8_pack(const V8<T>& x, float s, float y, bool quick) {
-    u64 w = 0;
+    template <typename T> __device__ __forceinline__ u64 pack(const V8<T>& x) const {
+        u64 w = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w |= (u64)q8_byte((float)x[j], s, y, quick) << (8 * j);
-    return w;
-}
+        for (int j = 0; j < 8; ++j) {
+            const float v = (float)x[j], q = v * y;
+            w |= (u64)(__float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, s, v), y, q) + 12582912.0f) & 0xffu) << (8 * j);
+        }
+        return w;
+    }
+    template <typename T> __device__ __forceinline__ u64 pack_slowly(const V8<T>& x) const {
+        u64 w = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w |= (u64)((u32)(int)fminf(fmaxf(__builtin_rintf((float)x[j] / s), -127.0f), 127.0f) & 0xffu) << (8 * j);
+        return live ? w : 0;
+    }
+};
 
-// One row by one wave: K elements of xr -> bytes at qr, of which [K, ldq) become zeros with pad; returns the scale.  The row is read once while it fits
-// the registers.
-template <typename T> __device__ __forceinline__ float q8_row(const T* xr, int K, signed char* qr, long long ldq, bool pad) {
-    const int l = threadIdx.x & 63, chunks = (K + 7) / 8;
-    V8<T> kept[Q8_KEPT];
+// One row by LANES lanes (`i`: this lane's place among them): K elements of xr -> bytes at qr, of which [K, ldq) become zeros with pad; returns the scale.
+// Up to KEPT chunks a lane stay in registers between the row's maximum and its bytes; longer rows are read again.  Whole chunks, the cut one and
+// the divisors that need a true division take paths of their own: unrolled together they did not fit the instruction cache.
+template <typename T, int LANES, int KEPT> __device__ __forceinline__ float q8_row(const T* xr, int K, signed char* qr, long long ldq, bool pad, int i) {
+    const int whole = K / 8, cut = K % 8 && whole % LANES == i ? whole : -1;
+    V8<T> kept[KEPT], end = {};
     float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < Q8_KEPT; ++i)
-        if (i * 64 < chunks) {
-            const int c = i * 64 + l;
-            kept[i] = c < chunks ? q8_load<T>(xr, c, K) : V8<T>{};
-        }
-#pragma unroll
-    for (int i = 0; i < Q8_KEPT; ++i)
-        if (i * 64 < chunks) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, q8_size((float)kept[i][j]));
-        }
-    for (int c = Q8_KEPT * 64 + l; c < chunks; c += 64) {
-        const V8<T> v = q8_load<T>(xr, c, K);
+    auto larger = [&](const V8<T>& v) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, q8_size((float)v[j]));
-    }
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float s = top == __builtin_inff() ? __builtin_nanf("") : top / 127.0f;
-    const bool live = s > 0.0f, quick = s > 1e-30f && (__float_as_uint(s) & 0x7fffff) != 0x7fffff;
-    const float y = 1.0f / s;
-    auto put = [&](int c, const V8<T>& v) {
-        const u64 w = live ? q8_pack<T>(v, s, y, quick) : 0;
-        if (8 * c + 8 <= K || pad) __builtin_memcpy(qr + 8 * c, &w, 8);      // (what lies behind the row's end quantises from zeros)
-        else
-            for (int j = 0; 8 * c + j < K; ++j) qr[8 * c + j] = (signed char)(w >> (8 * j));
     };
 #pragma unroll
-    for (int i = 0; i < Q8_KEPT; ++i)
-        if (i * 64 + l < chunks) put(i * 64 + l, kept[i]);
-    for (int c = Q8_KEPT * 64 + l; c < chunks; c += 64) put(c, q8_load<T>(xr, c, K));
+    for (int t = 0; t < KEPT; ++t)
+        if (t * LANES < whole) kept[t] = t * LANES + i < whole ? q8_load<T>(xr, t * LANES + i) : V8<T>{};
+    if (cut >= 0) {
+        end = q8_load_cut<T>(xr, cut, K);
+        larger(end);
+    }
+#pragma unroll
+    for (int t = 0; t < KEPT; ++t)
+        if (t * LANES < whole) larger(kept[t]);
+#pragma unroll 1
+    for (int c = KEPT * LANES + i; c < whole; c += LANES) larger(q8_load<T>(xr, c));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const Q8Divisor d(top);
+    auto put = [&](int c, u64 w) { __builtin_memcpy(qr + 8 * c, &w, 8); };
+    int from = i;
+    if (d.quick) {
+#pragma unroll
+        for (int t = 0; t < KEPT; ++t)
+            if (t * LANES + i < whole) put(t * LANES + i, d.pack<T>(kept[t]));
+        from = KEPT * LANES + i;
+    }
+#pragma unroll 1
+    for (int c = from; c < whole; c += LANES) {
+        const V8<T> v = q8_load<T>(xr, c);
+        put(c, d.quick ? d.pack<T>(v) : d.pack_slowly<T>(v));
+    }
+    if (cut >= 0) {
+        const u64 w = d.pack_slowly<T>(end);                               // (what lies behind the row's end quantises from zeros)
+        if (pad) put(cut, w);
+        else
+            for (int j = 0; 8 * cut + j < K; ++j) qr[8 * cut + j] = (signed char)(w >> (8 * j));
+    }
     if (pad)
-        for (long long c = chunks + l; c < ldq / 8; c += 64) *(u64*)(qr + 8 * c) = 0;
-    return s;
+        for (long long c = (K + 7) / 8 + i; c < ldq / 8; c += LANES) put((int)c, 0);
+    return d.s;
 }
 
 // Rows of x -> 8-bit rows (ldq bytes apart; pad: bytes [K, ldq) become zeros) and their scales.  One wave per row.
@@ -118,7 +144,7 @@ __global__ __launch_bounds__(256) void mfar_quantize_rows_kernel(const T* x, lon
         return;
     }
     if (row >= M) return;
-    const float s = q8_row<T>(x + (long long)row * ldx, K, q + (long long)row * ldq, ldq, pad != 0);
+    const float s = q8_row<T, 64, Q8_KEPT>(x + (long long)row * ldx, K, q + (long long)row * ldq, ldq, pad != 0, l);
     if (l == 0) scale[row] = s;
 }
 
@@ -187,9 +213,13 @@ __global__ __launch_bounds__(256) void mfar_int8_few_kernel(const Int8Params p, 
         for (int u = 0; u < 4; ++u) a[u] = q8_weights(p, n0 + (l & 31), k0 + u * 128 + 16 * half);
     };
     fetch(wave * 32);
-    for (int r = wave; r < p.M; r += 4) {
-        const float s = q8_row<X>(x + (long long)r * ldx, p.K, q8_lds + r * pitch, p.Kp, true);
-        if (l == 0) scales[r] = s;
+    // 16 lanes a row, 16 rows at a time
+    for (int r0 = 0; r0 < p.M; r0 += 16) {
+        const int r = r0 + (int)threadIdx.x / 16;
+        if (r < p.M) {
+            const float s = q8_row<X, 16, 8>(x + (long long)r * ldx, p.K, q8_lds + r * pitch, p.Kp, true, threadIdx.x & 15);
+            if ((threadIdx.x & 15) == 0) scales[r] = s;
+        }
     }
     __syncthreads();
     const signed char* row = q8_lds + min(l & 31, p.M - 1) * pitch + 16 * half;
