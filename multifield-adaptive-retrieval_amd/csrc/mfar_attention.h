@@ -373,6 +373,12 @@ __device__ __forceinline__ void at_softmax(f32x16 (&s)[N], T* vt, AtSoftmax& m, 
 // log2-sum of a query: -inf if it saw nothing
 __device__ __forceinline__ float at_lse(float base, float sum) { return sum == 0.0f ? -__builtin_inff() : base + __log2f(sum); }
 
+// x as fp32 rounded it: a product that is converted to fp16 in the same instruction rounds once, and what is left of x would be taken from another
+// rounding than the one that was stored
+__device__ __forceinline__ float at_rounded(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 __device__ __forceinline__ float at_norm(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }   // no keys: zeros; NaN stays
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
@@ -422,12 +428,18 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     const int q0 = place.tile * AT_COLS + wave * 32;
     const long long at = (((long long)b * p.Lq + q0) * p.H + h) * p.D;
     void* lds = at_lds + wave * at_out_bytes<T, DP>();
-    at_store<T, DP>((T*)p.out + at, (long long)p.H * p.D, p.Lq - q0, acc, f, p.D, lds);
-    if (KEEP) {
+    if (!KEEP) {
+        at_store<T, DP>((T*)p.out + at, (long long)p.H * p.D, p.Lq - q0, acc, f, p.D, lds);
+    } else {
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[dt][i] = acc[dt][i] * f - (float)(T)(acc[dt][i] * f);
+            for (int i = 0; i < 16; ++i) acc[dt][i] = at_rounded(acc[dt][i] * f);
+        at_store<T, DP>((T*)p.out + at, (long long)p.H * p.D, p.Lq - q0, acc, 1.0f, p.D, lds);
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[dt][i] -= (float)(T)acc[dt][i];
         at_store<T, DP>((T*)p.out_lo + at, (long long)p.H * p.D, p.Lq - q0, acc, 1.0f, p.D, lds);
     }
     if (p.lse && live && half == 0) p.lse[((long long)b * p.H + h) * p.Lq + q] = at_lse(m.base, sum);
@@ -442,6 +454,7 @@ struct AttnSplit {
     int splits;
 };
 template <typename T> __device__ __forceinline__ void at_write(const AttnParams& p, bool keep, long long at, float x) {
+    x = at_rounded(x);
     const T y = (T)x;
     ((T*)p.out)[at] = y;
     if (keep) ((T*)p.out_lo)[at] = (T)(x - (float)y);

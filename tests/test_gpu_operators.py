@@ -197,6 +197,24 @@ def test_attention_gradients_of_small_and_large_losses(size):
         assert bool(((a - b).abs() <= tol).all()), n
 
 
+@pytest.mark.parametrize("dtype,B,Lq", [("fp16", 32, 300), ("bf16", 32, 300), ("fp16", 8, 300), ("fp16", 200, 20)])
+def test_attention_output_is_kept_to_twice_its_type(dtype, B, Lq):
+    """What the forward pass leaves for the backward one: out and what its rounding dropped, together as exact as P in two parts makes them (u^2 of P|V|,
+    fp32 elsewhere) -- for every single element."""
+    from helpers.operator_refs import U32, attention_ref, half_step
+    from mfar.modeling.attention import _borders, _forward
+    q, k, v, table, _ = _attention_inputs(16, B, Lq, 24, 3, 64, dtype)          # few keys: an output is not much smaller than P|V|
+    out, lo, lse, _ = _forward(q, k, v, table, None, 0, False, _borders(32, False, 128), 1.0, True)
+    want, loose = attention_ref(q, k, v, table, None, False, 128, 0, 1.0)["out"]
+    u = half_step(q.dtype)
+    # the reference's bound without its two roundings to the type: 64 half steps of fp32 times 1 + the largest score (under 9 here), of P|V|, which
+    # `loose` = u |out| + (u + f) P|V| + .. holds at least u times
+    pv = loose / u
+    tiny = 2.0 ** -24 if dtype == "fp16" else 0.0
+    err = (out.double() + lo.double() - want).abs()
+    assert bool((err <= (4 * u * u + 64 * 10 * U32) * pv + tiny).all()), float((err / pv).max())
+
+
 def test_attention_is_reproducible_and_follows_the_current_stream():
     q, k, v, table, dout = _attention_inputs(10, 3, 300, 300, 4, 64, "bf16")
     a = _run_attention(q, k, v, table, dout)
