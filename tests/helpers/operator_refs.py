@@ -72,8 +72,8 @@ def attention_ref(q, k, v, table, key_mask, causal, max_distance, start, scale, 
     res["dq"] = (back(dq), back(u * dq.abs() + scale * (eS @ kd.abs()) + f * scale * (dS.abs() @ kd.abs()) + tiny))
     res["dk"] = (back(dk), back(u * dk.abs() + scale * (eS.transpose(2, 3).contiguous() @ qd.abs()) + f * scale * (dS.abs().transpose(2, 3).contiguous() @ qd.abs()) + tiny))
     res["dv"] = (back(dv), back(u * dv.abs() + (((u + f) * P + tiny).transpose(2, 3).contiguous() @ g.abs()) + tiny))
-    one = torch.nn.functional.one_hot(at, table.shape[0]).double()       # [B, Lq, Lk, buckets]
-    summed = lambda x: torch.einsum("bhqk,bqkn->nh", x.masked_fill(~seen, 0.0), one)   # noqa: E731
+    def summed(x):                                                       # [buckets, H]
+        return torch.stack([torch.bincount(at.reshape(-1), weights=x.masked_fill(~seen, 0.0)[:, h].reshape(-1), minlength=table.shape[0]) for h in range(H)], 1)
     res["dtable"] = (summed(dS), summed(raw + f * dS.abs()) + 1e-30)
     return res
 

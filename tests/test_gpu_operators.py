@@ -59,6 +59,47 @@ def test_attention_head_sizes_that_fill_no_chunk(D):
     _check_attention(q, k, v, table, dout)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("B,Lq,Lk,H,D,causal", [(130, 150, 150, 1, 64, False), (40, 213, 213, 4, 40, True), (3, 300, 200, 40, 128, False), (270, 40, 70, 1, 32, True),
+                                                (1, 8200, 4300, 4, 64, False)])
+def test_attention_of_batches_that_fill_the_gpu(dtype, B, Lq, Lk, H, D, causal):
+    """256 blocks of 128 queries and more: the kernel of large batches, forward and backward, with ragged key masks and over 4096 keys."""
+    print(f"attention {dtype} {B} {Lq} {Lk} {H} {D} {causal}", flush=True)
+    if dtype == "fp32" and Lk > 4096:
+        pytest.skip("the 64-bit reference of 4 x 8200 x 4300 is made for two types only")
+    q, k, v, table, dout = _attention_inputs(17, B, Lq, Lk, H, D, dtype)
+    lens = torch.randint(0, Lk + 1, (B,), generator=_gen(18), device="cuda")
+    lens[0] = Lk
+    mask = torch.arange(Lk, device="cuda") < lens[:, None]
+    if not causal:
+        mask[:, 5] = False
+    _check_attention(q, k, v, table, dout, mask=mask, causal=causal)
+    if Lk <= 4096:
+        _check_attention(q, k, v, table, dout, causal=causal, start=3)
+    k2, v2 = k.clone(), v.clone()
+    k2[~mask], v2[~mask] = float("nan"), float("inf")
+    a = _run_attention(q, k, v, table, dout, key_mask=mask, causal=causal)
+    b = _run_attention(q, k2, v2, table, dout, key_mask=mask, causal=causal)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+@pytest.mark.parametrize("B", [5, 300])
+def test_attention_layouts_give_the_same_bits_in_large_batches(B):
+    L, H, D = 70, 3, 32
+    q, k, v, table, dout = _attention_inputs(19, B, L, L, H, D, "bf16")
+    want = _run_attention(q, k, v, table, dout)
+    packed = torch.stack([q, k, v], dim=2)
+    got = _run_attention(packed[:, :, 0], packed[:, :, 1], packed[:, :, 2], table, dout)
+    heads = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    got2 = _run_attention(*heads, table, dout.transpose(1, 2).contiguous().transpose(1, 2))
+    mask = torch.rand(B, L, generator=_gen(20), device="cuda") < 0.6
+    shifted = torch.zeros(B, L + 3, dtype=torch.bool, device="cuda")
+    shifted[:, 3:] = mask                                                  # rows that start on no particular byte
+    m1, m2 = _run_attention(q, k, v, table, dout, key_mask=mask), _run_attention(q, k, v, table, dout, key_mask=shifted[:, 3:])
+    for a, b in ((want, got), (want, got2), (m1, m2)):
+        assert all(torch.equal(a[n], b[n]) for n in a)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "fp16"])
 def test_attention_masks_holes_empty_rows_and_poison(dtype):
     """Right-padded, scattered, fully hidden and single-key masks; hidden keys hold NaN, infinities and the type's lowest value."""
