@@ -446,7 +446,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
 }
 
 // ---- forward, few queries (short texts, a decoder's next token, small batches): the work of 32 queries is divided over the keys --------------------
-// Tiles of 32 keys go to the waves in turn, 4 waves a block and `splits` blocks per (batch, head): K straight into fragments, V through LDS of the
+// Tiles of 32 keys go to the waves in turn, 4 waves a block and `splits` blocks per (batch, head): K and V in whole rows through LDS of the
 // wave's own, no barrier in the loop, the next tile's loads in flight.  The waves' partial softmaxes are joined in LDS, the blocks' in a second
 // launch, both in a fixed order.  Bound by reading K and V.
 struct AttnSplit {
@@ -460,12 +460,16 @@ template <typename T> __device__ __forceinline__ void at_write(const AttnParams&
     if (keep) ((T*)p.out_lo)[at] = (T)(x - (float)y);
 }
 
+// LDS of the waves' tiles, and behind the loop of their partial outputs
+template <typename T, int DP> constexpr int at_few_bytes() { return 4 * DP * 32 * (sizeof(T) == 4 ? 8 : 4); }
+
 template <typename T, int DP, bool KEEP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_attn_few_kernel(const AttnParams p, const AttnSplit sp) {
     extern __shared__ __align__(16) unsigned char at_lds[];
-    T* vt = (T*)at_lds + wave_index() * 32 * DP;
+    T* vt = (T*)at_lds + wave_index() * 64 * DP;                           // the wave's V and K tiles
+    T* kt = vt + 32 * DP;
     float* part = (float*)at_lds;                                          // [4 waves][DP][32], behind the loop
-    float* stat = part + 4 * DP * 32;                                      // [4 waves][2][32]
+    float* stat = (float*)(at_lds + at_few_bytes<T, DP>());                // [4 waves][2][32]
     float* lut = stat + 4 * 64;
     const int b = blockIdx.z, h = blockIdx.y, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5, qi = l & 31;
     const int q0 = (int)blockIdx.x / sp.splits * 32, part_of = (int)blockIdx.x % sp.splits, q = q0 + qi;
@@ -478,22 +482,19 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     const T* vb = (const T*)p.v + b * p.v_b + h * p.v_h;
     const unsigned char* mask = p.mask ? p.mask + (long long)b * p.mask_b : nullptr;
     const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
-    V8<T> qf[DP / 16], kf[DP / 16], vr[NV];
+    V8<T> qf[DP / 16], kr[NV], vr[NV];
     bool on = false;
     const int step = sp.splits * 4 * 32;
     int k0 = (part_of * 4 + wave) * 32;
     const bool vin = (l % CH) * 8 < p.D;
     auto fetch = [&]() {
-        const int key = min(k0 + (l & 31), end - 1);
-        const T* row = kb + (long long)key * p.k_l;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) kf[s] = at_load<T>(row, true, s, p.D);
 #pragma unroll
         for (int t = 0; t < NV; ++t) {
-            const int r = min(k0 + (t * 64 + l) / CH, end - 1);
-            vr[t] = *(const V8<T>*)(vb + (long long)r * p.v_l + (vin ? (l % CH) * 8 : 0));
+            const int r = min(k0 + (t * 64 + l) / CH, end - 1), d = vin ? (l % CH) * 8 : 0;
+            kr[t] = *(const V8<T>*)(kb + (long long)r * p.k_l + d);
+            vr[t] = *(const V8<T>*)(vb + (long long)r * p.v_l + d);
         }
-        on = k0 + (l & 31) < end && (!mask || mask[key] != 0);
+        on = k0 + (l & 31) < end && (!mask || mask[min(k0 + (l & 31), end - 1)] != 0);
     };
     if (k0 < end) fetch();
 #pragma unroll
@@ -506,18 +507,20 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     while (k0 < end) {
         const u32 seen = (u32)__ballot(on);
         const int row0 = k0;
-        f32x16 s[1] = {};
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) s[0] = mma(kf[d], qf[d], s[0]);
 #pragma unroll
         for (int t = 0; t < NV; ++t) {
             const int r = (t * 64 + l) / CH;
-            *(V8<T>*)at_at<T, DP>(vt, r, l % CH) = vin && ((seen >> r) & 1) ? vr[t] : V8<T>{};
+            const bool shown = vin && ((seen >> r) & 1);
+            *(V8<T>*)at_at<T, DP>(kt, r, l % CH) = shown ? kr[t] : V8<T>{};
+            *(V8<T>*)at_at<T, DP>(vt, r, l % CH) = shown ? vr[t] : V8<T>{};
         }
         k0 += step;
         if (k0 < end) fetch();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        f32x16 s[1] = {};
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) s[0] = mma(at_rows<T, DP>(kt, 0, d), qf[d], s[0]);
         if (seen) {
             at_bias<1>(s[0], lut, p.sat, c, row0, col, start + q0, p.causal != 0, run.base);
             if (seen != ~0u) at_hide(s[0], seen);

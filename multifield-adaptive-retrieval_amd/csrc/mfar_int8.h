@@ -188,9 +188,13 @@ __device__ __forceinline__ i32x4 q8_weights(const Int8Params& p, int n, int k) {
         if (at + 16 <= end) {
             __builtin_memcpy(&w, p.wq + at, 16);
         } else {
-            signed char tail[16];
-            for (int j = 0; j < 16; ++j) tail[j] = at + j < end ? p.wq[at + j] : (signed char)0;
-            __builtin_memcpy(&w, tail, 16);
+            u64 part[2] = {0, 0};
+#pragma unroll 1
+            for (long long j = end - 1; j >= at; --j) {                     // from the last byte down, each pushing the others up
+                part[1] = part[1] << 8 | part[0] >> 56;
+                part[0] = part[0] << 8 | (unsigned char)p.wq[j];
+            }
+            __builtin_memcpy(&w, part, 16);
         }
     }
     return w;

@@ -141,7 +141,7 @@ int64_t split_rows(const mfar_attention* a) { return (int64_t)a->B * a->Lq * a->
 int64_t split_bytes(const mfar_attention* a) { return few_queries(a) && key_splits(a) > 1 ? split_rows(a) * (a->D + 2) * 4 : 0; }
 
 template <typename T, int DP, bool KEEP> int attention_few(const AttnParams& p, const AttnSplit& sp, hipStream_t st) {
-    const size_t lds = 4ull * DP * 32 * 4 + 4 * 64 * 4 + lut_bytes(p);     // (the V tiles, 4 * 32 * DP elements, lie in its first part)
+    const size_t lds = at_few_bytes<T, DP>() + 4 * 64 * 4 + lut_bytes(p);
     int rc = launch<mfar_attn_few_kernel<T, DP, KEEP>>("mfar_attn_few_kernel", dim3(cdiv(p.Lq, 32) * sp.splits, p.H, p.B), lds, st, p, sp);
     if (rc == MFAR_OK && sp.splits > 1)
         rc = launch<mfar_attn_join_kernel<T, KEEP>>("mfar_attn_join_kernel", dim3(cdiv((int64_t)p.B * p.Lq * p.H, 4)), 0, st, p, sp);
