@@ -131,10 +131,11 @@ template <typename T, int DP> constexpr size_t tile_bytes(bool backward) {
 int64_t dexp_bytes(const mfar_attention* a) { return a->dtype == MFAR_DTYPE_F16 ? ((int64_t)a->B * a->H * cdiv(a->Lq, AT_COLS) * 4 + 15) / 16 * 16 : 0; }
 size_t lut_bytes(const AttnParams& p) { return (size_t)(2 * (p.sat + AT_EDGE) + 1) * 4; }
 
-// Up to 32 queries, and batches of fewer than 256 blocks of 128 (one per CU), take the kernel that divides the keys over waves and blocks
-// (7 x 4 heads x 213 fp32: 25 us as 56 blocks); a block gets at least 8 tiles of 32 keys, and there are
-// no more than about two blocks per CU (16 x 12 heads over ragged caches of 4097: 32.9 us; three 33.8, four 36.6, eight 39.9; full caches: 47, 44, 47, 51).
-bool few_queries(const mfar_attention* a) { return a->Lq <= 32 || cdiv(a->Lq, AT_COLS) * a->B * a->H < 256; }
+// Up to 32 queries, and batches of fewer than 128 blocks of 128 queries, take the kernel that divides the keys over waves and blocks (7 x 4 heads x 213
+// fp32, 56 blocks: 12.4 us against 25.3; about even at 192: 1 x 12 x 2048 fp16 42 against 49, 4 x 12 x 512 17.5 against 15.4).  A block gets at least
+// 8 tiles of 32 keys, and there are no more than about two blocks per CU (16 x 12 heads over ragged caches of 4097: 32.9 us; three 33.8, four
+// 36.6, eight 39.9; full caches: 47, 44, 47, 51).
+bool few_queries(const mfar_attention* a) { return a->Lq <= 32 || cdiv(a->Lq, AT_COLS) * a->B * a->H < 128; }
 int key_splits(const mfar_attention* a) {
     return (int)std::max<int64_t>(1, std::min(cdiv(512, cdiv(a->Lq, 32) * a->B * a->H), cdiv(a->Lk, 8 * 32)));
 }
