@@ -28,6 +28,12 @@ def attention_dropout(stack: torch.nn.Module) -> float:
     return max(float(b.layer[0].SelfAttention.dropout) for b in stack.block)
 
 
+def _held(h: torch.Tensor) -> torch.Tensor:
+    """Hidden states of an fp16 model stay within the type, as the stock blocks keep them: a sum past the largest value would be infinite, and NaN
+    from the next norm on."""
+    return h if h.dtype != torch.float16 else h.clamp(-65504.0, 65504.0)
+
+
 def t5_encoder_forward(stack: torch.nn.Module, input_ids: torch.Tensor, attention_mask: torch.Tensor) -> torch.Tensor:
     """Token ids [B, L] and their mask (0: padding) -> hidden states [B, L, d].  No attention weight is dropped."""
     mask = attention_mask.ne(0)
@@ -42,6 +48,6 @@ def t5_encoder_forward(stack: torch.nn.Module, input_ids: torch.Tensor, attentio
         x = layer.layer_norm(h)
         heads = (B, L, att.n_heads, att.key_value_proj_dim)
         o = relative_bias_attention(att.q(x).view(heads), att.k(x).view(heads), att.v(x).view(heads), table, key_mask=mask, max_distance=max_distance)
-        h = h + layer.dropout(att.o(o.reshape(B, L, -1)))
-        h = block.layer[-1](h)                                            # the feed-forward with its norm, dropout and residual
+        h = _held(h + layer.dropout(att.o(o.reshape(B, L, -1))))
+        h = _held(block.layer[-1](h))                                          # the feed-forward with its norm, dropout and residual
     return stack.dropout(stack.final_layer_norm(h))

@@ -61,6 +61,23 @@ def test_fused_t5_forward_under_autocast(dtype):
     assert err(fused) <= 2 * err(stock) + 1e-6, (err(fused), err(stock))
 
 
+def test_fused_t5_in_fp16_stays_within_the_type():
+    """An fp16 model whose sums of hidden states pass the type's largest value: held there, as the stock blocks hold them, not infinite and then NaN."""
+    enc = _t5().half().eval()
+    seen = []
+    with torch.no_grad():
+        for block in enc.auto_model.encoder.block[:2]:
+            o = block.layer[0].SelfAttention.o
+            o.weight.fill_(6e4)
+            o.register_forward_hook(lambda m, i, out: seen.append(bool(out.isinf().any())))
+        f = _features(enc, _texts(9, 60))
+        stock = enc(f)["sentence_embedding"]
+        enc.use_fused_attention()
+        seen.clear()
+        fused = enc(f)["sentence_embedding"]
+    assert any(seen) and bool(stock.isfinite().all()) and bool(fused.isfinite().all())
+
+
 def test_fused_t5_gradients_are_the_stock_gradients():
     """Every parameter's gradient, the bias table's among them, in fp32 (no dropout)."""
     enc = _t5()
