@@ -512,7 +512,7 @@ int mfar_pipeline_lists(mfar_pipeline* p, int64_t ticket, int64_t* field_ids, fl
  */
 typedef struct mfar_attention {
     int32_t dtype;                          /* MFAR_DTYPE_F32 / BF16 / F16: q, k, v, out and their gradients */
-    int32_t B, Lq, Lk, H, D;                /* D: multiple of 8, <= 128; B, H <= 65535 */
+    int32_t B, Lq, Lk, H, D;                /* D: multiple of 8, <= 128; B, H <= 65535; lengths <= 2^30 - 256; B H (max length / 128) < 2^24 */
     int32_t causal, n_buckets, n_borders;   /* n_buckets <= 256 (even unless causal) */
     float scale;
     const int32_t* borders;                 /* HOST [n_borders], ascending: n_borders = side - side / 2 - 1; last (or each) <= 1023 */
@@ -543,7 +543,8 @@ int mfar_attention_backward(int device, const mfar_attention* a, void* stream); 
  *   mfar_quantize_rows: scale[m] = max|x[m]| / 127, q[m] = rint(x[m] / scale[m]), ties to even; rows of q ldq bytes apart.  A row of zeros gets
  *   scale 0, a row with an infinity or NaN scale NaN and zeros.
  *   mfar_int8_linear: y = quantize_rows(x) wq' scaled by both scales (+ bias), rounded once to y's type.
- * x [M, K] rows ldx elements apart; wq [N, K] contiguous, 16-byte aligned; w_scale [N]; bias [N] fp32 or NULL; y [M, N] contiguous, of any of the three types.  K <= 131072.
+ * x [M, K] rows ldx elements apart; wq [N, K] contiguous, 16-byte aligned; w_scale [N]; bias [N] fp32 or NULL; y [M, N] contiguous, of any of the three types.
+ * K <= 131072; M, N <= 2^23.
  */
 int mfar_quantize_rows(int device, const void* x, int dtype, int64_t ldx, int64_t M, int K, int8_t* q, int64_t ldq, float* scale, void* stream);
 int64_t mfar_int8_linear_workspace_bytes(int64_t M, int K, int N);
@@ -553,7 +554,7 @@ int mfar_int8_linear(int device, const void* x, int dtype, int64_t ldx, int64_t 
 /*
  * Distillation from a teacher's top scores: p = softmax(scores / tau) over a row's ids >= 0, q = softmax(student / tau) over its N columns;
  * loss[t] = tau^2 KL(p || q).  A row without ids: loss and gradient 0.  An id >= N: the row's loss and gradient are NaN.  An id may repeat.
- * student [T, N] rows ld elements apart; ids [T, K] int64, scores [T, K] fp32, K <= 1024; prob [T, K] and stat [T, 2] are kept for the backward
+ * student [T, N] rows ld elements apart, T < 2^24, N <= 2^30; ids [T, K] int64, scores [T, K] fp32, K <= 1024; tau in 1e-18..1e18; prob [T, K] and stat [T, 2] are kept for the backward
  * pass; dstudent [T, N] contiguous, of the student's type; dloss [T].
  */
 int64_t mfar_distill_workspace_bytes(int64_t T, int64_t N);

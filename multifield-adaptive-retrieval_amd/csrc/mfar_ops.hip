@@ -45,6 +45,7 @@ struct OnDevice {
     } while (0)
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+constexpr int64_t MAX_BLOCKS = 1 << 24;       // of 256 threads: a launch counts its threads in 32 bits
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int type_size(int dtype) { return dtype == MFAR_DTYPE_F32 ? 4 : (dtype == MFAR_DTYPE_BF16 || dtype == MFAR_DTYPE_F16) ? 2 : 0; }
 
@@ -78,8 +79,8 @@ int check_attention(const mfar_attention* a, bool backward) {
     if (!es) return bad("dtype must be F32, BF16 or F16");
     if (a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 1 || a->B > 65535 || a->H > 65535) return bad("B, Lq, Lk must be >= 0, H >= 1, B and H <= 65535");
     if (a->D < 8 || a->D > 128 || a->D % 8) return bad("D must be a multiple of 8, at most 128");
-    if (cdiv((int64_t)a->B * a->H, 8) * 8 * cdiv(std::max(a->Lq, a->Lk), AT_COLS) > 0x7fffffff) return bad("too many tiles for one launch");
-    if (a->Lq > (1 << 30) || a->Lk > (1 << 30)) return bad("at most 2^30 queries and keys");
+    if (a->Lq > (1 << 30) - 256 || a->Lk > (1 << 30) - 256) return bad("at most 2^30 - 256 queries and keys");     // positions and their differences fit 32 bits
+    if (cdiv((int64_t)a->B * a->H, 8) * 8 * cdiv(std::max(a->Lq, a->Lk), AT_COLS) >= MAX_BLOCKS) return bad("batch, heads and tiles of 128 queries or keys: under 2^24 blocks");
     if (a->q_start < -(1 << 30) || a->q_start > (1 << 30)) return bad("q_start out of range");
     if (a->n_buckets < 2 || a->n_buckets > 256 || (!a->causal && (a->n_buckets % 2 || a->n_buckets < 4))) return bad("n_buckets must be 2..256, even and >= 4 unless causal");
     const int side = a->causal ? a->n_buckets : a->n_buckets / 2, each = side / 2;
@@ -111,7 +112,7 @@ AttnParams attention_params(const mfar_attention* a) {
     p.do_b = a->do_b, p.do_l = a->do_l, p.do_h = a->do_h;
     p.table = a->table, p.mask = a->key_mask, p.mask_b = a->mask_b, p.start_ptr = a->q_start_each, p.start = a->q_start, p.lse = a->lse;
     p.B = a->B, p.Lq = a->Lq, p.Lk = a->Lk, p.H = a->H, p.D = a->D, p.causal = a->causal != 0, p.scale = a->scale;
-        p.n_buckets = a->n_buckets, p.n_side = a->causal ? a->n_buckets : a->n_buckets / 2;
+    p.n_buckets = a->n_buckets, p.n_side = a->causal ? a->n_buckets : a->n_buckets / 2;
     const int each = p.n_side / 2;
     p.sat = a->n_borders ? a->borders[a->n_borders - 1] : each;
     for (int m = 0; m < p.n_side; ++m) p.first[m] = (short)(m <= each ? m : a->borders[m - each - 1]);
@@ -202,9 +203,9 @@ template <typename T> int distill_backward(const DistillParams& p, hipStream_t s
 }
 int check_distill(const void* x, int dtype, int64_t ld, int64_t T, int64_t N, const int64_t* ids, int K, float tau) {
     if (!type_size(dtype)) return bad("dtype must be F32, BF16 or F16");
-    if (T < 0 || T > 0x7fffffff || N < 1 || N > (1 << 30)) return bad("T must be 0..2^31 - 1, N 1..2^30");
+    if (T < 0 || T >= MAX_BLOCKS || N < 1 || N > (1 << 30)) return bad("T must be 0..2^24 - 1, N 1..2^30");
     if (K < 1 || K > DI_MAX_K) return bad("K must be 1..1024");
-    if (!(tau > 0.0f) || tau > 3.0e38f) return bad("the temperature must be positive and finite");
+    if (!(tau >= 1e-18f && tau <= 1e18f)) return bad("the temperature must be 1e-18..1e18");                 // its square and log2(e) over it are fp32 numbers
     if (T && (!x || !ids)) return bad("NULL tensor");
     if (T > 1 && ld < 0) return bad("rows must not run backwards");
     return MFAR_OK;

@@ -122,7 +122,7 @@ def topk_distillation(student: torch.Tensor, teacher_ids: torch.Tensor, teacher_
 
     student [T, N] float32 / float16 / bfloat16 on the GPU; teacher_ids [T, K] int64 or int32 columns, K <= 1024, negative: no entry (short
     lists); teacher_scores [T, K], used in fp32, no gradient.  A row without entries has loss 0 and gradient 0; an id past the last column
-    makes its row NaN; a repeated id adds up."""
+    makes its row NaN; a repeated id adds up.  Fewer than 2^24 rows; temperature 1e-18 to 1e18."""
     _native.op_device(student, teacher_ids, teacher_scores)
     if student.dim() != 2 or student.shape[1] < 1 or student.shape[1] > 2 ** 30:
         raise ValueError(f"expected student scores [T, N], 1 <= N <= 2^30, got {tuple(student.shape)}")
@@ -132,8 +132,8 @@ def topk_distillation(student: torch.Tensor, teacher_ids: torch.Tensor, teacher_
         raise ValueError(f"a teacher's list has 1 to 1024 entries, got {teacher_ids.shape[1]}")
     if teacher_scores.shape != teacher_ids.shape or not teacher_scores.is_floating_point():
         raise ValueError(f"expected float teacher_scores {tuple(teacher_ids.shape)}, got {teacher_scores.dtype} {tuple(teacher_scores.shape)}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"the temperature must be positive and finite, got {temperature}")
+    if not 1e-18 <= temperature <= 1e18:
+        raise ValueError(f"the temperature must be 1e-18 to 1e18, got {temperature}")
     _native.op_dtype(student)
     return _TopKDistillation.apply(student, teacher_ids.to(torch.int64).contiguous(), teacher_scores.detach().float().contiguous(), float(temperature))
 

@@ -37,7 +37,7 @@ def _borders(*values):
     (dict(D=12), "D must"), (dict(D=136), "D must"), (dict(Lq=2 ** 30 + 1), "2\\^30"), (dict(q_start=2 ** 30 + 1), "q_start"), (dict(n_buckets=1), "n_buckets"),
     (dict(n_buckets=31), "n_buckets"), (dict(n_buckets=258), "n_buckets"), (dict(n_borders=6), "n_borders"), (dict(causal=1), "n_borders"), (dict(q=None), "NULL"),
     (dict(table=None), "NULL"), (dict(v=None), "NULL"), (dict(out=None), "NULL"), (dict(k_l=4), "strides"), (dict(v_h=65), "strides"), (dict(q=4104), "aligned"),
-    (dict(out_lo=4100), "aligned"),
+    (dict(out_lo=4100), "aligned"), (dict(Lk=2 ** 30), "2\\^30"), (dict(B=65535, H=257), "2\\^24"), (dict(B=128, H=16, Lq=2 ** 21), "2\\^24"),
 ])
 def test_attention_refusals_at_the_c_abi(change, what):
     from mfar import _native
@@ -89,8 +89,8 @@ def test_int8_and_distillation_refusals_at_the_c_abi():
     assert L.mfar_int8_linear(*[0 if i in (4,) else v for i, v in enumerate(ok)]) == 0
     assert L.mfar_distill_workspace_bytes(4, 0) == -1 and L.mfar_distill_workspace_bytes(2, 10 ** 6) > 0 and L.mfar_distill_workspace_bytes(5000, 100) == 0
     ok = [0, P, 0, 1000, 4, 1000, P, P, 8, 1.0, P, P, P, P, 1 << 20, None]
-    for i, v in ((1, None), (2, 4), (3, -5), (4, -1), (4, 2 ** 31), (5, 0), (5, 2 ** 30 + 1), (6, None), (7, None), (8, 0), (8, 1025), (9, 0.0), (9, -1.0),
-                 (9, math.inf), (9, math.nan), (10, None), (11, None), (12, None)):
+    for i, v in ((1, None), (2, 4), (3, -5), (4, -1), (4, 2 ** 31), (4, 2 ** 24), (5, 0), (5, 2 ** 30 + 1), (6, None), (7, None), (8, 0), (8, 1025), (9, 0.0), (9, -1.0),
+                 (9, math.inf), (9, math.nan), (9, 1e-19), (9, 2e18), (10, None), (11, None), (12, None)):
         args = list(ok)
         args[i] = v
         assert L.mfar_distill_forward(*args) == -1, (i, v)
