@@ -158,12 +158,12 @@ template <typename T, int DP> __device__ __forceinline__ V8<T> at_cols(T* tile, 
     }
     return x;
 }
-// B fragment straight from memory: column = row `row` of the matrix, dims 16 s + 8 half + j
+// B fragment straight from memory: column = row `row` of the matrix, dims 16 s + 8 half + j; zeros where the row is not live or has no such dim.
+// (`row` may be read in any case: loads without branches are all in flight at once)
 template <typename T> __device__ __forceinline__ V8<T> at_load(const T* row, bool live, int s, int D) {
     const int d = 16 * s + 8 * ((threadIdx.x & 63) >> 5);
-    V8<T> x = {};
-    if (live && d < D) x = *(const V8<T>*)(row + d);
-    return x;
+    const V8<T> x = *(const V8<T>*)(row + (d < D ? d : 0));
+    return live && d < D ? x : V8<T>{};
 }
 template <typename T> __device__ __forceinline__ V8<T> at_pack(const f32x16& t, int m) {
     V8<T> x;
@@ -250,19 +250,20 @@ template <typename T, int DP, bool BACKWARD, typename A, typename F>
 __device__ __forceinline__ void at_for_tiles(const AttnParams& p, int b, int h, int end, T* tiles, A&& ahead, F&& step) {
     constexpr int S = at_stages(sizeof(T), DP, BACKWARD), SIZE = AT_TILE * DP;
     const AtStream<T, DP> ks((const T*)p.k + b * p.k_b + h * p.k_h, p.k_l, end, p.D), vs((const T*)p.v + b * p.v_b + h * p.v_h, p.v_l, end, p.D);
-    if (end <= 0) ahead();
-    for (int base = 0; base < end; base += 64 * AT_TILE) {
-        const u64 words = at_words(p, b, base, end);
-        u64 left = __ballot(words != 0);                                   // the same in every wave
-        int t = left ? __builtin_ctzll(left) : 0, slot = 0;
-        if (base) __syncthreads();                                         // (the readers of the 4096 keys before are done)
-        if (left) {
-            ks.load(base + t * AT_TILE, tiles);
-            vs.load(base + t * AT_TILE, tiles + SIZE);
-        }
-        if (base == 0) ahead();
-        if (!left) continue;
-        while (true) {
+    u64 words = 0, left = 0;                                               // left: the same in every wave
+    int t = 0, slot = 0;
+    auto begin = [&](int base) {
+        words = at_words(p, b, base, end);
+        left = __ballot(words != 0);
+        if (!left) return;
+        t = __builtin_ctzll(left), slot = 0;
+        ks.load(base + t * AT_TILE, tiles);
+        vs.load(base + t * AT_TILE, tiles + SIZE);
+    };
+    if (end > 0) begin(0);
+    ahead();
+    for (int base = 0; base < end; ) {
+        while (left) {
             const int k0 = base + t * AT_TILE;
             const u64 bits = read_lane(words, t);
             T *kt = tiles + slot * 2 * SIZE, *vt = kt + SIZE;
@@ -288,6 +289,11 @@ __device__ __forceinline__ void at_for_tiles(const AttnParams& p, int b, int h, 
                 __syncthreads();
                 next();
             }
+        }
+        base += 64 * AT_TILE;
+        if (base < end) {
+            __syncthreads();                                               // (the readers of the 4096 keys before are done)
+            begin(base);
         }
     }
 }
@@ -401,7 +407,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
         const int last = start + min(p.Lq, (place.tile + 1) * AT_COLS);      // one past the last query's position
         end = min(end, max(last, 0));
     }
-    const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
+    const T* qrow = (const T*)p.q + b * p.q_b + (long long)(live ? q : 0) * p.q_l + h * p.q_h;
     V8<T> qf[DP / 16];
     f32x16 acc[DP / 32] = {};
     AtSoftmax m;
@@ -481,7 +487,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     const T* kb = (const T*)p.k + b * p.k_b + h * p.k_h;
     const T* vb = (const T*)p.v + b * p.v_b + h * p.v_h;
     const unsigned char* mask = p.mask ? p.mask + (long long)b * p.mask_b : nullptr;
-    const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
+    const T* qrow = (const T*)p.q + b * p.q_b + (long long)(live ? q : 0) * p.q_l + h * p.q_h;
     V8<T> qf[DP / 16], kr[NV], vr[NV];
     bool on = false;
     const int step = sp.splits * 4 * 32;
@@ -596,20 +602,36 @@ template <typename T, bool KEEP> __global__ __launch_bounds__(AT_BLOCK) void mfa
 }
 
 // Sums along the diagonals of a 32 x 32 tile (lanes: queries, registers: keys) times the lane's f, added to sums[key - query]; by one wave, in memory of
-// its own.  Element (key r, query q) goes to place r - q + 31 of row r of a 32 x 64 buffer: a diagonal is a column there, and what no element reaches
-// stays the zero it was set to once.  Every lane adds up a column and adds the sum to its distance's place: no atomics (LDS float atomics took 205
-// cycles a wave here, 16 of them a tile).
-#define AT_SKEW (32 * 64)
+// its own.  A lane's registers come in runs of 4 rows: from the last row of a run up, the sum so far moves on by a query (a lane) and the next row is
+// added.  What leaves the run's half of the wave by that (query 0) enters the other half's upper end, at distances past the run's own, and is
+// kept apart (`off`).  The 8 runs of a tile, their distances in columns, lie in a buffer of 8 x 64 (what no run reaches stays the zero it was set to
+// once); every lane adds up a column and adds the sum to its distance's place.  No atomics (LDS float atomics took 205 cycles a wave here).
+#define AT_SKEW (8 * 64)
+__device__ __forceinline__ float at_next_lane(float x) {                    // lane n: lane n + 1's, the last lane: 0
+    return __uint_as_float((u32)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x130, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float at_next_lane_around(float x) {             // lane n: lane n + 1's, the last lane: the first's
+    return __uint_as_float((u32)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x134, 0xf, 0xf, true));
+}
 __device__ __forceinline__ void at_diagonals(const f32x16& s, float f, float* skew, float* sums) {
     const int l = threadIdx.x & 63, half = l >> 5, q = l & 31;
-    float* to = skew + 4 * half * 65 + 31 - q;
+    float *own = skew + 68 * half + 31 - q, *other = skew + 68 * (1 - half) + 63 - q;     // run g of a half: row 2 g + half, first key 8 g + 4 half
 #pragma unroll
-    for (int i = 0; i < 16; ++i) to[crow(i, 0) * 65] = s[i] * f;
+    for (int g = 0; g < 4; ++g) {
+        float sum = s[4 * g + 3] * f, off = 0.0f;
+#pragma unroll
+        for (int i = 2; i >= 0; --i) {
+            off = at_next_lane_around(q == 0 ? sum : off);
+            sum = s[4 * g + i] * f + at_next_lane(l == 32 ? 0.0f : sum);
+        }
+        own[136 * g] = sum;
+        if (q >= 29) other[136 * g] = off;
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     float t[2] = {};
 #pragma unroll
-    for (int r = 0; r < 32; ++r) t[r & 1] += skew[r * 64 + l];
+    for (int r = 0; r < 8; ++r) t[r & 1] += skew[r * 64 + l];
     if (l < 63) sums[l - 31] += t[0] + t[1];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -625,7 +647,7 @@ __device__ __forceinline__ float at_pow2(int e) { return __uint_as_float((u32)(e
 
 // ---- backward: dQ, the bias gradient, D ---------------------------------------------------------------------------------------------------
 template <typename T, int DP>
-__global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_attn_dq_kernel(const AttnParams p) {
+__global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_attn_dq_kernel(const AttnParams p) {
     AtPlace place;
     if (!at_place(p, (p.Lq + AT_COLS - 1) / AT_COLS, place)) return;
     extern __shared__ __align__(16) unsigned char at_lds[];
@@ -642,9 +664,9 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const int col = start + q, col_lo = start + place.tile * AT_COLS + wave * 32;
     int end = p.Lk;
     if (p.causal) end = min(end, max(start + min(p.Lq, (place.tile + 1) * AT_COLS), 0));
-    const T* qrow = (const T*)p.q + b * p.q_b + (long long)q * p.q_l + h * p.q_h;
-    const T* grow = (const T*)p.dout + b * p.do_b + (long long)q * p.do_l + h * p.do_h;
-    const long long orow = (((long long)b * p.Lq + q) * p.H + h) * p.D, srow = ((long long)b * p.H + h) * p.Lq + q;
+    const T* qrow = (const T*)p.q + b * p.q_b + (long long)(live ? q : 0) * p.q_l + h * p.q_h;
+    const T* grow = (const T*)p.dout + b * p.do_b + (long long)(live ? q : 0) * p.do_l + h * p.do_h;
+    const long long orow = (((long long)b * p.Lq + (live ? q : 0)) * p.H + h) * p.D, srow = ((long long)b * p.H + h) * p.Lq + q;
     V8<T> qf[DP / 16], gf[DP / 16];
     float dsum = 0.0f, lse = 0.0f, up = 1.0f, down = 1.0f;                 // up: the power of two dS is scaled by, down: back
     f32x16 acc[DP / 32] = {};
@@ -656,7 +678,8 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
         for (int s = 0; s < DP / 16; ++s) {
             qf[s] = at_load<T>(qrow, live, s, p.D);
             gf[s] = at_load<T>(grow, live, s, p.D);
-            const V8<T> o = at_load<T>((const T*)p.o + orow, live, s, p.D), lo = at_load<T>((const T*)p.o_lo + orow, live && p.o_lo, s, p.D);
+            const V8<T> o = at_load<T>((const T*)p.o + orow, live, s, p.D);
+            const V8<T> lo = sizeof(T) == 2 ? at_load<T>((const T*)(p.o_lo ? p.o_lo : p.o) + orow, live && p.o_lo, s, p.D) : V8<T>{};
 #pragma unroll
             for (int j = 0; j < 8; ++j) dsum = __builtin_fmaf((float)gf[s][j], (float)o[j] + (float)lo[j], dsum);
         }
@@ -732,16 +755,17 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
             hist[i] = t;
         }
         __syncthreads();
-        // a bucket holds the distances [lo, hi) of one side
+        // a bucket holds the distances [lo, hi) of one side; 8 lanes add them up
         const int q_tiles = (p.Lq + AT_COLS - 1) / AT_COLS;
         float* to = p.dpart + ((long long)(b * q_tiles + place.tile) * p.H + h) * p.n_buckets;
-        for (int n = threadIdx.x; n < p.n_buckets; n += AT_BLOCK) {
+        for (int n = threadIdx.x / 8; n < p.n_buckets; n += AT_BLOCK / 8) {
             const bool front = n >= p.n_side;
             const int m = n - (front ? p.n_side : 0);
             const int lo = max((int)p.first[m], front ? 1 : 0), hi = m == p.n_side - 1 ? p.sat + AT_EDGE + 1 : p.first[m + 1];   // (distance 0 counts as behind)
             float t = 0.0f;
-            for (int d = lo; d < hi; ++d) t += hist[(front ? d : -d) + p.sat + AT_EDGE];
-            to[n] = t;
+            for (int d = lo + (threadIdx.x & 7); d < hi; d += 8) t += hist[(front ? d : -d) + p.sat + AT_EDGE];
+            for (int o = 1; o < 8; o <<= 1) t += __shfl_xor(t, o);
+            if ((threadIdx.x & 7) == 0) to[n] = t;
         }
     }
 }
@@ -809,11 +833,12 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     if (first < p.Lq) fetch(first, 0);
     const T* krow = (const T*)p.k + b * p.k_b + (long long)key * p.k_l + h * p.k_h;
     const T* vrow = (const T*)p.v + b * p.v_b + (long long)key * p.v_l + h * p.v_h;
-    V8<T> kf[DP / 16], vf[DP / 16];
+    V8<T> kf[DP / 16], vf[DP / 16];                                         // (hidden keys' rows are not read)
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
-        kf[s] = at_load<T>(krow, seen, s, p.D);
-        vf[s] = at_load<T>(vrow, seen, s, p.D);
+        const int d = 16 * s + 8 * half;
+        kf[s] = vf[s] = V8<T>{};
+        if (seen && d < p.D) kf[s] = *(const V8<T>*)(krow + d), vf[s] = *(const V8<T>*)(vrow + d);
     }
     at_lut(p, lut, h);
     for (int q0 = first; q0 < p.Lq; q0 += AT_TILE) {
