@@ -180,7 +180,7 @@ template <typename T> __device__ __forceinline__ V8<T> at_pack_lo(const f32x16& 
 }
 // O' tiles of a wave (lane: one of 32 rows of the result, registers: dims) -> n rows of a [.., D] matrix `stride` elements apart, through LDS of the
 // wave's own (at_out_bytes), 128 bytes of a row at a time, so that a row leaves in runs of whole cache lines (8 bytes a lane of 32 rows
-// straight from the registers: 83 us instead of 78 for the encode).
+// straight from the registers: 5 us more for the encode's 73).
 template <typename T, int DP> constexpr int at_out_dims() { return DP * (int)sizeof(T) < 128 ? DP : 128 / (int)sizeof(T); }
 template <typename T, int DP> constexpr int at_out_bytes() { return 32 * (at_out_dims<T, DP>() * (int)sizeof(T) + 16); }
 template <typename T, int DP> __device__ __forceinline__ void at_store(T* out, long long stride, int n, const f32x16* acc, float f, int D, void* lds) {
@@ -646,6 +646,8 @@ __device__ __forceinline__ int at_exponent(float largest) {
 __device__ __forceinline__ float at_pow2(int e) { return __uint_as_float((u32)(e + 127) << 23); }
 
 // ---- backward: dQ, the bias gradient, D ---------------------------------------------------------------------------------------------------
+// Bound by the vector unit (exponentials, bias, diagonal sums) with the matrix unit behind it at long lengths, by the first loads of a block at short ones:
+// three blocks a CU (32 x 512 x 12 heads x 64 fp16: 84 us, two blocks 94; of it the bias gradient 16; 4 x 4096: 372 us, 830 TFLOP/s).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_attn_dq_kernel(const AttnParams p) {
     AtPlace place;
@@ -785,6 +787,8 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dtable_kernel(const float*
 }
 
 // ---- backward: dK, dV (keys in lanes) -------------------------------------------------------------------------------------------------------
+// Two blocks a CU: what a third would leave of the registers does not hold two accumulators, K and V (32 x 512 x 12 heads x 64 fp16: 83 us against 95 to
+// 103; 4 x 4096: 465 against 520 to 560).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_attn_dkv_kernel(const AttnParams p) {
     AtPlace place;

@@ -1,6 +1,8 @@
 // mfar_int8.h -- 8-bit linear layer: y[m][n] = (sum_k xq[m][k] wq[n][k]) * xs[m] * ws[n] + bias[n]
 //
-//   xs[m] = max_k |x[m][k]| / 127, xq = rint(x / xs) (ties to even)          one scale per token, computed on the fly
+//   xs[m] = max_k |x[m][k]| (1 / 127), xq = rint(x / xs) (ties to even)          one scale per token, computed on the fly
+// (1 / 127 rounded to fp32, then the product: within an ulp of the quotient, and what a division by a constant number gives in torch, so that the
+// elementary operations there find the same bytes)
 //   ws[n], wq: one scale per output channel, laid out once by the caller
 // The integer sums are exact (|sum| <= 127^2 K < 2^31 for K <= 131072); rounding happens in the scales and once at the end.
 // A row of zeros has scale 0 and gives the bias; a row with an infinity or NaN has scale NaN and gives NaN.
@@ -51,7 +53,7 @@ struct Q8Divisor {
     float s, y;
     bool live, quick;
     __device__ __forceinline__ explicit Q8Divisor(float top) {
-        s = top == __builtin_inff() ? __builtin_nanf("") : top / 127.0f;
+        s = top == __builtin_inff() ? __builtin_nanf("") : top * (1.0f / 127.0f);
         live = s > 0.0f;
         quick = s > 1e-30f && (__float_as_uint(s) & 0x7fffff) != 0x7fffff;
         y = 1.0f / s;
@@ -202,7 +204,7 @@ __device__ __forceinline__ i32x4 q8_weights(const Int8Params& p, int n, int k) {
 
 // ---- up to 32 tokens: quantising and product in one launch ------------------------------------------------------------------------------------
 // Every block quantises all rows into LDS (they are few) while its first weights are on their way, then multiplies 32 channels by them, k divided over
-// the waves.  12 x 768 x 768: one launch of 6 us for two of 9.
+// the waves.  12 x 768 x 768: one launch of 8 us for two of 9 together.
 #define Q8_FEW_ROWS 32
 #define Q8_FEW_K 2048
 template <typename T, typename X>

@@ -28,8 +28,8 @@ def _check(x: torch.Tensor) -> None:
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """x [..., K] float32 / float16 / bfloat16 -> (q int8 [..., K], scale fp32 [...]): scale = max|row| / 127, q = rint(row / scale), ties to
-    even.  A row of zeros has scale 0; a row with an infinity or NaN has scale NaN and zeros."""
+    """x [..., K] float32 / float16 / bfloat16 -> (q int8 [..., K], scale fp32 [...]): scale = max|row| times 1 / 127 (both rounded to fp32),
+    q = rint(row / scale), ties to even.  A row of zeros has scale 0; a row with an infinity or NaN has scale NaN and zeros."""
     dev = _native.op_device(x)
     _check(x)
     K = x.shape[-1]

@@ -311,10 +311,10 @@ def test_attention_empty_sizes():
 
 # ---- 8-bit linear -----------------------------------------------------------------------------------------------------------------------
 def _quantize_ref(x):
-    # both quotients rounded to fp32 once: a quotient of two fp32 numbers in 64 bits, rounded to 32, is the correctly rounded one (53 >= 2 * 24 + 2
-    # bits), which torch's own fp32 division by a number is not (it multiplies by the reciprocal)
+    # the product and the quotient rounded to fp32 once: a quotient of two fp32 numbers in 64 bits, rounded to 32, is the correctly rounded one
+    # (53 >= 2 * 24 + 2 bits)
     xd = x.double()
-    s = (xd.abs().amax(-1, keepdim=True) / 127).float()
+    s = (xd.abs().amax(-1, keepdim=True) * float(torch.tensor(1.0) / 127)).float()      # (exact in 64 bits, then rounded)
     n = (xd / torch.where(s > 0, s, torch.ones_like(s)).double()).float()
     return torch.round(n).clamp(-127, 127).to(torch.int8), s[..., 0]
 
@@ -327,6 +327,16 @@ def test_quantize_rows(dtype, M, K):
     q, s = quantize_rows(x)
     wq, ws = _quantize_ref(x)
     assert torch.equal(s, ws) and torch.equal(q, wq)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_quantize_rows_as_elementary_operations_do(dtype):
+    """The same bytes and scales: one that fell on the other side of a tie would be a whole step off."""
+    from mfar.modeling.quantized import quantize_rows
+    x = torch.randn(20000, 1003, generator=_gen(33), device="cuda").to(TYPES[dtype])
+    q, s = quantize_rows(x)
+    scale = x.float().abs().amax(1) / 127
+    assert torch.equal(s, scale) and torch.equal(q, torch.round(x.float() / scale[:, None]).to(torch.int8))
 
 
 def test_quantize_rows_ties_zeros_and_poison():
