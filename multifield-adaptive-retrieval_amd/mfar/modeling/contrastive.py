@@ -220,7 +220,7 @@ class RetrievalTrainingModule(torch.nn.Module):
         max_len = int(self.encoder.get_max_seq_length())
         tb = os.environ.get("MFAR_ENCODE_TOKEN_BUDGET", "1")             # 0: always dev_batch_size texts; 1: the default; n > 1: n tokens
         budget = 0 if tb == "0" else (int(tb) if tb.isdigit() and int(tb) > 1 else bs * max_len)
-        # Precision of the corpus-encode forwards (SURVEY 8 f1): `self.encode_precision`, overridden by MFAR_ENCODE_AUTOCAST=fp32|fp16|bf16|int8.
+        # Precision of the corpus-encode forwards: `self.encode_precision`, overridden by MFAR_ENCODE_AUTOCAST=fp32|fp16|bf16|int8.
         # The reference encodes the corpus outside its precision plugin (which wraps the steps, not on_test_epoch_start) but with
         # torch.set_float32_matmul_precision("high") (train.py:67, mask_fields.py:52): fp32 matmuls may run with 10-bit-mantissa inputs on
         # its hardware.  gfx950 has no such fp32 mode; fp16 autocast IS that precision here (11-bit significand into fp32 accumulators):
