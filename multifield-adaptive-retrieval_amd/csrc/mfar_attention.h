@@ -11,6 +11,9 @@
 // summed index is free, mfar_ops_device.h).  The backward pass uses the same trick twice: queries in lanes for dQ (and the bias gradient),
 // keys in lanes for dK / dV; each recomputes P from the stored log2-sum of the forward pass.  No float atomics on shared addresses: results
 // do not change from run to run.
+// P and dS are rounded to the inputs' type on their way into a product (the matrix unit takes nothing wider at its rate): half a step each, independent
+// from key to key, which adds to dQ and dK about what the rounding of those results does (2.9e-4 from the 64-bit gradient for 2.1e-4 in fp16; bf16
+// over two keys 2.9e-3 for 1.7e-3).  Sums stay in fp32, the table's gradient takes dS unrounded.
 //
 // The bias of a (query, key) pair depends on k - pos(q) alone and is constant beyond `sat` (the first distance of the last bucket): a table
 // of 2 sat + 1 values per head lives in LDS, and a tile whose distances all lie beyond sat adds one constant.
