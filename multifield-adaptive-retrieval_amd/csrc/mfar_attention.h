@@ -18,6 +18,8 @@
 // The bias of a (query, key) pair depends on k - pos(q) alone and is constant beyond `sat` (the first distance of the last bucket): a table
 // of 2 sat + 1 values per head lives in LDS, and a tile whose distances all lie beyond sat adds one constant.
 #pragma once
+#include <type_traits>
+
 #include "mfar_ops_device.h"
 
 #define AT_BLOCK 256      // 4 waves, 32 query (key) columns each
@@ -45,7 +47,6 @@ struct AttnParams {
     const int* start_ptr;        // [B] position of the first query among the keys, or NULL
     float *lse, *drow;           // [B, H, Lq], log2 units
     float* dpart;                // [blocks, H, n_buckets] partial bias gradients, or NULL
-    int* dexp;                   // [B, H, tiles of 128 queries] largest exponent of dO (fp16)
     int start, B, Lq, Lk, H, D, causal, n_buckets, n_side, sat;
     float scale;
     short first[129 * 2];        // first distance of each bucket of a side
@@ -643,13 +644,32 @@ __device__ __forceinline__ void at_diagonals(const f32x16& s, float f, float* sk
     __builtin_amdgcn_wave_barrier();
 }
 
-// fp16 holds nothing under 2^-24: the score gradients dS are scaled by a power of two on their way into a product and back behind it, by each
-// query's own (dQ: queries in lanes) or by that of the (batch, head)'s largest dO (dK: summed over queries).  dP - D takes the factor in an fma.
-__device__ __forceinline__ int at_exponent(float largest) {
-    const int e = (int)((__float_as_uint(largest) >> 23) & 255) - 127;
-    return e > 100 ? 0 : max(e, -100);                                      // (infinities and NaN as they are)
-}
+// Score gradients on their way into an fp16 product: dS is dO times V times P, more than fp16's range holds at either end.  Each lane's column (dQ: a
+// query's, dK: a key's) goes into the product times a power of two of its own, taken back behind the sums.  The column's first tile sets it, its
+// largest entry to 2^6; when an entry passes 2^15 it is set anew and the sums so far move with it.  What then lies under fp16's normal numbers is
+// under 2^-20 of the column's largest.  (32 x 512 x 12 heads x 64: dK / dV as without it, dQ 84 -> 87 us; 4 x 4096: dQ 388 -> 403.)
+struct AtFit {
+    float scale = 1.0f, cap = 0.0f;                                         // cap: 2^15; 0 until an entry is met
+    __device__ __forceinline__ float back() const { return __uint_as_float(0x7f000000u - __float_as_uint(scale)); }   // 1 / scale
+};
 __device__ __forceinline__ float at_pow2(int e) { return __uint_as_float((u32)(e + 127) << 23); }
+// s: the tile's entries times m.scale.  Returns what the column's sums were multiplied by.
+template <int N> __device__ __forceinline__ float at_fit(f32x16& s, AtFit& m, f32x16 (&acc)[N]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, __builtin_fabsf(s[i]));
+    if (!__any(top > m.cap)) return 1.0f;
+    top = max_halves(top);                                                  // (a column lies in both halves)
+    const int e = (int)(__float_as_uint(top) >> 23) - 127;                  // infinite: left as it is; under 2^-60 the results are zeros
+    const float keep = top > m.cap && e < 128 ? at_pow2(6 - max(e, -60)) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= keep;
+#pragma unroll
+    for (int dt = 0; dt < N; ++dt) acc[dt] *= keep;
+    m.scale *= keep;
+    if (top > m.cap) m.cap = 0x1p15f;
+    return keep;
+}
 
 // ---- backward: dQ, the bias gradient, D ---------------------------------------------------------------------------------------------------
 // Bound by the vector unit (exponentials, bias, diagonal sums) with the matrix unit behind it at long lengths, by the first loads of a block at short ones:
@@ -661,7 +681,6 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     extern __shared__ __align__(16) unsigned char at_lds[];
     T* tiles = (T*)at_lds;
     float* lut = (float*)(tiles + at_stages(sizeof(T), DP, true) * 2 * AT_TILE * DP);
-    __shared__ int exps[4];
     const int n_lut = at_lut_size(p.sat);
     float* hist = lut + n_lut;                                             // [4 waves][n_lut] sums of dS by distance
     float* skew = hist + 4 * n_lut;                                        // [4 waves][AT_SKEW]
@@ -676,7 +695,9 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     const T* grow = (const T*)p.dout + b * p.do_b + (long long)(live ? q : 0) * p.do_l + h * p.do_h;
     const long long orow = (((long long)b * p.Lq + (live ? q : 0)) * p.H + h) * p.D, srow = ((long long)b * p.H + h) * p.Lq + q;
     V8<T> qf[DP / 16], gf[DP / 16];
-    float dsum = 0.0f, lse = 0.0f, up = 1.0f, down = 1.0f;                 // up: the power of two dS is scaled by, down: back
+    float dsum = 0.0f, lse = 0.0f;
+    constexpr bool FIT = std::is_same<T, _Float16>::value;
+    AtFit fit;
     f32x16 acc[DP / 32] = {};
     float far_lo = 0.0f, far_hi = 0.0f;
     const float c = p.scale * LOG2E;
@@ -696,19 +717,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
             for (int i = threadIdx.x; i < 4 * (n_lut + AT_SKEW); i += AT_BLOCK) hist[i] = 0.0f;
         dsum = sum_halves(dsum);
         if (live && half == 0) p.drow[srow] = dsum;
-        if (sizeof(T) == 2 && p.dexp) {
-            float largest = 0.0f;
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) largest = fmaxf(largest, __builtin_fabsf((float)gf[s][j]));
-            int e = at_exponent(max_halves(largest));
-            up = at_pow2(-e), down = at_pow2(e);
-            for (int o = 1; o < 32; o <<= 1) e = max(e, __shfl_xor(e, o));
-            if (l == 0) exps[wave] = e;
-        }
         if (!live || lse == -__builtin_inff()) lse = __builtin_inff();      // no keys: P = exp2(-inf) = 0 everywhere
-        dsum *= up;
     }, [&](int k0, u64 bits, T* kt, T* vt) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -723,7 +732,11 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
             const u32 shown = (u32)(bits >> (32 * t));
             if (shown != ~0u) at_hide(s, shown);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i]) * __builtin_fmaf(dp[i], up, -dsum);
+            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i]) * (FIT ? __builtin_fmaf(dp[i], fit.scale, -dsum * fit.scale) : dp[i] - dsum);
+            if (FIT) {
+                const float keep = at_fit(s, fit, acc);
+                far_lo *= keep, far_hi *= keep;
+            }
             if (p.dpart) {
                 if (row0 - col_lo - 31 >= p.sat) {
 #pragma unroll
@@ -732,7 +745,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
 #pragma unroll
                     for (int i = 0; i < 16; ++i) far_lo += s[i];
                 } else {
-                    at_diagonals(s, down, skew + wave * AT_SKEW, hist + wave * n_lut + (row0 - col_lo) + p.sat + AT_EDGE);
+                    at_diagonals(s, FIT ? fit.back() : 1.0f, skew + wave * AT_SKEW, hist + wave * n_lut + (row0 - col_lo) + p.sat + AT_EDGE);
                 }
             }
 #pragma unroll
@@ -743,10 +756,9 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
     });
     __syncthreads();                                                       // (the tiles' memory is free)
     const int q0 = place.tile * AT_COLS + wave * 32;
-    at_store<T, DP>((T*)p.dq + (((long long)b * p.Lq + q0) * p.H + h) * p.D, (long long)p.H * p.D, p.Lq - q0, acc, p.scale * down, p.D, at_lds + wave * at_out_bytes<T, DP>());
-    if (sizeof(T) == 2 && p.dexp && threadIdx.x == 0) p.dexp[((long long)b * p.H + h) * ((p.Lq + AT_COLS - 1) / AT_COLS) + place.tile] = max(max(exps[0], exps[1]), max(exps[2], exps[3]));
+    at_store<T, DP>((T*)p.dq + (((long long)b * p.Lq + q0) * p.H + h) * p.D, (long long)p.H * p.D, p.Lq - q0, acc, p.scale * (FIT ? fit.back() : 1.0f), p.D, at_lds + wave * at_out_bytes<T, DP>());
     if (p.dpart) {
-        far_lo *= down, far_hi *= down;
+        if (FIT) far_lo *= fit.back(), far_hi *= fit.back();
         for (int o = 1; o < 64; o <<= 1) {
             far_lo += __shfl_xor(far_lo, o);
             far_hi += __shfl_xor(far_hi, o);
@@ -802,7 +814,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     extern __shared__ __align__(16) unsigned char at_lds[];
     constexpr int S = at_stages(sizeof(T), DP, true), SIZE = AT_TILE * DP;
     T* tiles = (T*)at_lds;                                                 // [S][Q, dO][AT_TILE][DP]
-    float* stats = (float*)(tiles + S * 2 * SIZE);                          // [S][log2-sum, D][AT_TILE]
+    float* stats = (float*)(tiles + S * 2 * SIZE);                          // [S][log2-sum, -D][AT_TILE]
     float* lut = stats + S * 2 * AT_TILE;
     const int b = place.b, h = place.h, wave = wave_index(), l = threadIdx.x & 63, half = l >> 5;
     const int start = at_start(p, b);
@@ -819,21 +831,16 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     if (!__syncthreads_or(seen)) first = p.Lq;
     first = first / AT_TILE * AT_TILE;
     const AtStream<T, DP> qs(qb, p.q_l, p.Lq, p.D), gs(gb, p.do_l, p.Lq, p.D);
-    float mine = 0.0f, up = 1.0f, down = 1.0f;                              // thread i: entry i of the next tile's statistics
-    if (sizeof(T) == 2 && p.dexp) {
-        int e = -100;
-        const int n = (p.Lq + AT_COLS - 1) / AT_COLS;
-        for (int i = l; i < n; i += 64) e = max(e, p.dexp[((long long)b * p.H + h) * n + i]);
-        for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o));
-        up = at_pow2(-e), down = at_pow2(e);
-    }
+    float mine = 0.0f;                                                     // thread i: entry i of the next tile's statistics
+    constexpr bool FIT = std::is_same<T, _Float16>::value;
+    AtFit fit;
     auto fetch = [&](int q0, int slot) {
         qs.load(q0, tiles + slot * 2 * SIZE);
         gs.load(q0, tiles + slot * 2 * SIZE + SIZE);
         if (threadIdx.x < 2 * AT_TILE) {
             const int i = threadIdx.x % AT_TILE;
             const bool in = q0 + i < p.Lq, d = threadIdx.x >= AT_TILE;
-            mine = in ? (d ? p.drow[srow + q0 + i] * up : p.lse[srow + q0 + i]) : 0.0f;
+            mine = in ? (d ? -p.drow[srow + q0 + i] : p.lse[srow + q0 + i]) : 0.0f;
             // rows behind the last and rows that saw nothing: P = exp2(s - inf) = 0
             if (!d && (!in || mine == -__builtin_inff())) mine = __builtin_inff();
             stats[slot * 2 * AT_TILE + threadIdx.x] = mine;
@@ -864,7 +871,9 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
         if (S == 2) slot ^= 1;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            f32x16 s = {}, dp = {};
+            f32x16 s = {}, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] = rows[AT_TILE + 32 * t + crow(i, half)];      // -D: dP - D out of the product
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
                 s = mma(at_rows<T, DP>(qt, 32 * t, d), kf[d], s);
@@ -875,8 +884,9 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
             for (int i = 0; i < 16; ++i) {
                 const int r = 32 * t + crow(i, half);
                 s[i] = exp2_fast(s[i] - rows[r]);
-                dp[i] = s[i] * __builtin_fmaf(dp[i], up, -rows[AT_TILE + r]);
+                dp[i] *= FIT ? s[i] * fit.scale : s[i];
             }
+            if (FIT) at_fit(dp, fit, dk);
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -898,6 +908,6 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const int k0 = key0 + wave * 32;
     const long long at = (((long long)b * p.Lk + k0) * p.H + h) * p.D;
     void* lds = at_lds + wave * at_out_bytes<T, DP>();
-    at_store<T, DP>((T*)p.dk + at, (long long)p.H * p.D, p.Lk - k0, dk, p.scale * down, p.D, lds);
+    at_store<T, DP>((T*)p.dk + at, (long long)p.H * p.D, p.Lk - k0, dk, p.scale * (FIT ? fit.back() : 1.0f), p.D, lds);
     at_store<T, DP>((T*)p.dv + at, (long long)p.H * p.D, p.Lk - k0, dv, 1.0f, p.D, lds);
 }

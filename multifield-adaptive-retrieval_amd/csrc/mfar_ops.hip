@@ -129,7 +129,6 @@ template <typename T, int DP> constexpr size_t tile_bytes(bool backward) {
     static_assert(at_stages(sizeof(T), DP, true) * 2ull * AT_TILE * DP * sizeof(T) >= 4 * at_out_bytes<T, DP>());
     return n;
 }
-int64_t dexp_bytes(const mfar_attention* a) { return a->dtype == MFAR_DTYPE_F16 ? ((int64_t)a->B * a->H * cdiv(a->Lq, AT_COLS) * 4 + 15) / 16 * 16 : 0; }
 size_t lut_bytes(const AttnParams& p) { return (size_t)(2 * (p.sat + AT_EDGE) + 1) * 4; }
 
 // Up to 32 queries, and batches of fewer than 128 blocks of 128 queries, take the kernel that divides the keys over waves and blocks (7 x 4 heads x 213
@@ -268,7 +267,7 @@ extern "C" int64_t mfar_attention_workspace_bytes(const mfar_attention* a, int b
     if (rc != MFAR_OK) return rc;
     if (a->B == 0 || a->Lq == 0) return 0;
     if (!backward) return split_bytes(a);
-    return drow_bytes(a) + dexp_bytes(a) + (a->dtable ? cdiv(a->Lq, AT_COLS) * a->B * a->H * a->n_buckets * 4 : 0);
+    return drow_bytes(a) + (a->dtable ? cdiv(a->Lq, AT_COLS) * a->B * a->H * a->n_buckets * 4 : 0);
 }
 extern "C" int mfar_attention_forward(int device, const mfar_attention* a, void* stream) {
     int rc = check_attention(a, false);
@@ -288,8 +287,7 @@ extern "C" int mfar_attention_backward(int device, const mfar_attention* a, void
     ON_DEVICE(device);
     AttnParams p = attention_params(a);
     p.drow = (float*)a->workspace;
-    p.dexp = a->dtype == MFAR_DTYPE_F16 ? (int*)((char*)a->workspace + drow_bytes(a)) : nullptr;
-    p.dpart = a->dtable ? (float*)((char*)a->workspace + drow_bytes(a) + dexp_bytes(a)) : nullptr;
+    p.dpart = a->dtable ? (float*)((char*)a->workspace + drow_bytes(a)) : nullptr;
     return FOR_TYPE_AND_DIM(attention_backward, p, a->dtable, (hipStream_t)stream);
 }
 

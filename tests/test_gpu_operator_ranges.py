@@ -1,0 +1,103 @@
+"""GPU tests of the attention's gradients and outputs over the range of fp16's exponents: values that are large, probabilities that are small, keys that
+no query sees.  Held to the formula in 64 bits.
+
+Bounds: u is half a step of the type, f the 64 half steps of fp32 times 1 + the largest score that tests/helpers/operator_refs.py allows what stays in
+fp32.  P and dS are rounded to the type on their way into a product, each column of them (a query's for dQ, a key's for dK and dV) under a power of two of
+its own that puts its largest entry at 2^6 or more: entries in fp16's smallest numbers, whose half step is 2^-25, are off by at most 2^-31 of
+the column's largest.  No entry is allowed an absolute error; results alone are, half of fp16's smallest step."""
+import math
+
+import pytest
+import torch
+
+from helpers.operator_refs import U32, bucket_of, check, half_step
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _reference(q, k, v, table, dout, causal=False, scale=1.0, start=0):
+    """{name: (value, bound)} of out, dq, dk and dv in 64 bits; no masks.  Heads first inside."""
+    dt = q.dtype
+    u, small = half_step(dt), 2.0 ** -31 if dt == torch.float16 else 0.0
+    tiny = 2.0 ** -25 if dt == torch.float16 else 1e-37
+    t = lambda x: x.transpose(-1, -2).contiguous()   # noqa: E731
+    qd, kd, vd, g = (x.detach().double().transpose(1, 2).contiguous() for x in (q, k, v, dout))
+    Lq, Lk = qd.shape[2], kd.shape[2]
+    rel = torch.arange(Lk, device=q.device)[None] - torch.arange(Lq, device=q.device)[:, None] - start
+    lut = torch.tensor([bucket_of(d, table.shape[0], causal, 128) for d in range(-start - Lq, Lk + 1)], device=q.device)
+    S = scale * (qd @ t(kd)) + table.double()[lut[rel + start + Lq]].permute(2, 0, 1)
+    if causal:
+        S = S.masked_fill(rel > 0, -math.inf)
+    P = torch.softmax(S, 3)
+    f = 64 * U32 * (1 + float(S[torch.isfinite(S)].abs().max()))
+    out, dP = P @ vd, g @ t(vd)
+    D = (P * dP).sum(3, keepdim=True)
+    dS = P * (dP - D)
+    twice = 0.0 if dt == torch.float32 else 2 * u * u                     # D: from P in two parts and an output kept in two parts
+    eD = (twice + f) * (g.abs() * (P @ vd.abs())).sum(3, keepdim=True)
+    if dt == torch.float16:                                               # ... whose second parts may lie in the smallest numbers
+        eD = eD + 2 * (g.abs() * (2.0 ** -25 + 2.0 ** -31 * vd.abs().sum(2, keepdim=True))).sum(3, keepdim=True)
+    raw = f * P * (g.abs() @ t(vd.abs()) + D.abs()) + P * eD
+    e_q = raw + u * dS.abs() + small * (dS.abs() + raw).amax(3, keepdim=True)
+    e_k = raw + u * dS.abs() + small * (dS.abs() + raw).amax(2, keepdim=True)
+    e_p = (u + f) * P + small * P.amax(2, keepdim=True)
+    dq, dk, dv = scale * (dS @ kd), scale * (t(dS) @ qd), t(P) @ g
+    back = lambda x: x.transpose(1, 2)   # noqa: E731
+    return {"out": (back(out), back((u + small) * out.abs() + (u + f + small) * (P @ vd.abs()) + tiny)),
+            "dq": (back(dq), back(u * dq.abs() + scale * (e_q @ kd.abs() + f * (dS.abs() @ kd.abs())) + tiny)),
+            "dk": (back(dk), back(u * dk.abs() + scale * (t(e_k) @ qd.abs() + f * (t(dS.abs()) @ qd.abs())) + tiny)),
+            "dv": (back(dv), back(u * dv.abs() + t(e_p) @ g.abs() + tiny))}
+
+
+def _run(q, k, v, table, dout, **kw):
+    from mfar.modeling.attention import relative_bias_attention
+    leaves = [x.detach().clone().requires_grad_(True) for x in (q, k, v, table)]
+    out = relative_bias_attention(*leaves, **kw)
+    return dict(zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *torch.autograd.grad(out, leaves, dout))))
+
+
+def _hold(q, k, v, table, dout, **kw):
+    got = _run(q, k, v, table, dout, causal=kw.get("causal", False), scale=kw.get("scale", 1.0), q_start=kw.get("start", 0))
+    for name, (want, bound) in _reference(q, k, v, table, dout, **kw).items():
+        check(name, got[name], want, bound)
+    return got
+
+
+@pytest.mark.parametrize("D", [40, 64, 128])
+@pytest.mark.parametrize("size", [2000.0, 60000.0])
+def test_fp16_gradients_under_large_values(D, size):
+    """Two equally likely keys with values of opposite sign and a small gradient along them: dP is D times value times gradient, past fp16's largest number
+    once dO alone is brought near 1, while every gradient is an ordinary number."""
+    L, H = 2, 3
+    q, k = torch.zeros(1, L, H, D, device="cuda"), torch.full((1, L, H, D), 0.01, device="cuda")
+    q[..., 0] = 0.25
+    k[:, 1] *= -1
+    k[..., 0] = 0.0                                                       # equal scores
+    v = torch.full((1, L, H, D), size, device="cuda")
+    v[:, 1] *= -1
+    dout = torch.full((1, L, H, D), 2.0 / size, device="cuda")
+    x = [y.half() for y in (q, k, v)]
+    got = _hold(*x, torch.zeros(32, H, device="cuda"), dout.half())
+    assert all(bool(got[n].isfinite().all()) for n in got)
+    assert float(got["dq"].abs().max()) > 0.1 and float(got["dk"].abs().max()) > 1
+
+
+@pytest.mark.parametrize("B,Lq,Lk", [(2, 150, 150), (1, 300, 70), (1, 33, 200)])
+def test_fp16_gradients_of_rows_that_differ_in_size(B, Lq, Lk):
+    """Gradients from 2^-14 to 2^14 from query to query and values from 2^-10 to 2^10 from key to key, in any order along the tiles: every query's dQ and
+    every key's dK is held to its own size."""
+    H, D = 2, 64
+    g = _gen(31)
+    q = torch.randn(B, Lq, H, D, generator=g, device="cuda") * (1.0 / math.sqrt(D))
+    k, v, dout = (torch.randn(B, n, H, D, generator=g, device="cuda") for n in (Lk, Lk, Lq))
+    v = v * torch.exp2(torch.rand(B, Lk, H, 1, generator=g, device="cuda") * 20 - 10)
+    dout = dout * torch.exp2(torch.rand(B, Lq, H, 1, generator=g, device="cuda") * 28 - 14)
+    dout = dout * 2.0 ** -6                                               # (nothing past the type in the results themselves)
+    table = torch.randn(32, H, generator=g, device="cuda")
+    _hold(*(x.half() for x in (q, k * 0.05, v * 2.0 ** -4)), table, dout.half(), scale=20.0)
