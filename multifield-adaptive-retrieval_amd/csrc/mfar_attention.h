@@ -11,8 +11,8 @@
 // summed index is free, mfar_ops_device.h).  The backward pass uses the same trick twice: queries in lanes for dQ (and the bias gradient),
 // keys in lanes for dK / dV; each recomputes P from the stored log2-sum of the forward pass.  No float atomics on shared addresses: results
 // do not change from run to run.
-// P and dS are rounded to the inputs' type on their way into a product (the matrix unit takes nothing wider at its rate): half a step each, independent
-// from key to key, which adds to dQ and dK about what the rounding of those results does (2.9e-4 from the 64-bit gradient for 2.1e-4 in fp16; bf16
+// P and dS are rounded to the inputs' type on their way into a product (the matrix unit takes nothing wider at its rate): half a step each, in fp16
+// whatever their size (AtFit), independent from key to key, which adds to dQ and dK about what the rounding of those results does (2.9e-4 from the 64-bit gradient for 2.1e-4 in fp16; bf16
 // over two keys 2.9e-3 for 1.7e-3).  Sums stay in fp32, the table's gradient takes dS unrounded.
 //
 // The bias of a (query, key) pair depends on k - pos(q) alone and is constant beyond `sat` (the first distance of the last bucket): a table
@@ -644,28 +644,27 @@ __device__ __forceinline__ void at_diagonals(const f32x16& s, float f, float* sk
     __builtin_amdgcn_wave_barrier();
 }
 
-// Score gradients on their way into an fp16 product: dS is dO times V times P, more than fp16's range holds at either end.  Each lane's column (dQ: a
-// query's, dK: a key's) goes into the product times a power of two of its own, taken back behind the sums.  The column's first tile sets it, its
-// largest entry to 2^6; when an entry passes 2^15 it is set anew and the sums so far move with it.  What then lies under fp16's normal numbers is
-// under 2^-20 of the column's largest.  (32 x 512 x 12 heads x 64: dK / dV as without it, dQ 84 -> 87 us; 4 x 4096: dQ 388 -> 403.)
+// What the backward pass multiplies in fp16 does not stay within its range: dS is dO times V times P, and the P of a key that is unlikely for every
+// query is small throughout (fp16: exact from 2^-14, nothing under 2^-25).  So each lane's column (dQ: a query's dS; dK, dV: a key's dS and P)
+// goes into its product times a power of two of its own, taken back behind the sums.  The column's first tile sets it, its largest entry
+// to 2^6; when an entry passes 2^15 it is set anew and the sums so far move with it.  What then lies under fp16's normal numbers is under 2^-20 of the
+// column's largest.  (32 x 512 x 12 heads x 64, ragged: dQ 71 -> 75 us, dK / dV 78 -> 81; 4 x 4096: 390 -> 407 and 500 -> 530.)
 struct AtFit {
     float scale = 1.0f, cap = 0.0f;                                         // cap: 2^15; 0 until an entry is met
     __device__ __forceinline__ float back() const { return __uint_as_float(0x7f000000u - __float_as_uint(scale)); }   // 1 / scale
+    __device__ __forceinline__ float power() const { return (float)((int)(__float_as_uint(scale) >> 23) - 127); }     // log2 of it
 };
 __device__ __forceinline__ float at_pow2(int e) { return __uint_as_float((u32)(e + 127) << 23); }
-// s: the tile's entries times m.scale.  Returns what the column's sums were multiplied by.
-template <int N> __device__ __forceinline__ float at_fit(f32x16& s, AtFit& m, f32x16 (&acc)[N]) {
+__device__ __forceinline__ float at_largest(const f32x16& s) {
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, __builtin_fabsf(s[i]));
-    if (!__any(top > m.cap)) return 1.0f;
-    top = max_halves(top);                                                  // (a column lies in both halves)
+    return top;
+}
+// what a column whose tile has `top` as its largest is to be multiplied by, the sums so far with it
+__device__ __forceinline__ float at_refit(float top, AtFit& m) {
     const int e = (int)(__float_as_uint(top) >> 23) - 127;                  // infinite: left as it is; under 2^-60 the results are zeros
     const float keep = top > m.cap && e < 128 ? at_pow2(6 - max(e, -60)) : 1.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] *= keep;
-#pragma unroll
-    for (int dt = 0; dt < N; ++dt) acc[dt] *= keep;
     m.scale *= keep;
     if (top > m.cap) m.cap = 0x1p15f;
     return keep;
@@ -734,8 +733,13 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = exp2_fast(s[i]) * (FIT ? __builtin_fmaf(dp[i], fit.scale, -dsum * fit.scale) : dp[i] - dsum);
             if (FIT) {
-                const float keep = at_fit(s, fit, acc);
-                far_lo *= keep, far_hi *= keep;
+                const float top = at_largest(s);
+                if (__any(top > fit.cap)) {
+                    const float keep = at_refit(max_halves(top), fit);      // (a column lies in both halves)
+                    s *= keep, far_lo *= keep, far_hi *= keep;
+#pragma unroll
+                    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= keep;
+                }
             }
             if (p.dpart) {
                 if (row0 - col_lo - 31 >= p.sat) {
@@ -833,7 +837,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const AtStream<T, DP> qs(qb, p.q_l, p.Lq, p.D), gs(gb, p.do_l, p.Lq, p.D);
     float mine = 0.0f;                                                     // thread i: entry i of the next tile's statistics
     constexpr bool FIT = std::is_same<T, _Float16>::value;
-    AtFit fit;
+    AtFit fit, raise;                                                      // of dS; of P, which is small alone for a key that is unlikely for every query
     auto fetch = [&](int q0, int slot) {
         qs.load(q0, tiles + slot * 2 * SIZE);
         gs.load(q0, tiles + slot * 2 * SIZE + SIZE);
@@ -879,14 +883,21 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
                 s = mma(at_rows<T, DP>(qt, 32 * t, d), kf[d], s);
                 dp = mma(at_rows<T, DP>(gt, 32 * t, d), vf[d], dp);
             }
-            at_bias<-1>(s, lut, p.sat, c, start + q0 + 32 * t, key, col_lo, p.causal != 0, 0.0f);
+            at_bias<-1>(s, lut, p.sat, c, start + q0 + 32 * t, key, col_lo, p.causal != 0, FIT ? -raise.power() : 0.0f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int r = 32 * t + crow(i, half);
-                s[i] = exp2_fast(s[i] - rows[r]);
+                s[i] = exp2_fast(s[i] - rows[32 * t + crow(i, half)]);
                 dp[i] *= FIT ? s[i] * fit.scale : s[i];
             }
-            if (FIT) at_fit(dp, fit, dk);
+            if (FIT) {
+                const float top_p = at_largest(s), top = at_largest(dp);
+                if (__any(top_p > raise.cap || top > fit.cap)) {
+                    const float up = at_refit(max_halves(top_p), raise), keep = at_refit(max_halves(top) * up, fit) * up;
+                    s *= up, dp *= keep;
+#pragma unroll
+                    for (int dt = 0; dt < DP / 32; ++dt) dv[dt] *= up, dk[dt] *= keep;
+                }
+            }
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -908,6 +919,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const int k0 = key0 + wave * 32;
     const long long at = (((long long)b * p.Lk + k0) * p.H + h) * p.D;
     void* lds = at_lds + wave * at_out_bytes<T, DP>();
-    at_store<T, DP>((T*)p.dk + at, (long long)p.H * p.D, p.Lk - k0, dk, p.scale * (FIT ? fit.back() : 1.0f), p.D, lds);
-    at_store<T, DP>((T*)p.dv + at, (long long)p.H * p.D, p.Lk - k0, dv, 1.0f, p.D, lds);
+    const float lower = FIT ? raise.back() : 1.0f;
+    at_store<T, DP>((T*)p.dk + at, (long long)p.H * p.D, p.Lk - k0, dk, p.scale * (FIT ? fit.back() * lower : 1.0f), p.D, lds);
+    at_store<T, DP>((T*)p.dv + at, (long long)p.H * p.D, p.Lk - k0, dv, lower, p.D, lds);
 }

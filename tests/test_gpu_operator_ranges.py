@@ -101,3 +101,36 @@ def test_fp16_gradients_of_rows_that_differ_in_size(B, Lq, Lk):
     dout = dout * 2.0 ** -6                                               # (nothing past the type in the results themselves)
     table = torch.randn(32, H, generator=g, device="cuda")
     _hold(*(x.half() for x in (q, k * 0.05, v * 2.0 ** -4)), table, dout.half(), scale=20.0)
+
+
+@pytest.mark.parametrize("bias", [-8.0, -10.0, -12.0, -16.0, -30.0])
+@pytest.mark.parametrize("B,L,D", [(1, 512, 64), (1, 300, 128), (40, 200, 64)])
+def test_fp16_gradients_of_keys_with_small_probabilities(bias, B, L, D):
+    """Keys behind a learned bias that all but hides them still get gradients as exact as the type: P and dS of such a key are all small, none of them large
+    beside them.  dO is what a gradient scaler hands over (2^10 over a mean's)."""
+    H = 2
+    g = _gen(32)
+    q = torch.randn(B, L, H, D, generator=g, device="cuda") * (1.0 / math.sqrt(D))
+    k, v, dout = (torch.randn(B, L, H, D, generator=g, device="cuda") for _ in range(3))
+    table = torch.randn(32, H, generator=g, device="cuda")
+    table[16:] += bias                                                    # every key past the query, from near ones to the last bucket
+    x = [y.half() for y in (q, k, v, dout * 2.0 ** 10)]
+    x[3][:, L // 2:] = 0.0                                                # (the second half's queries count for nothing: its keys are seen through the bias only)
+    got = _hold(x[0], x[1], x[2], table, x[3])
+    want = _reference(x[0], x[1], x[2], table, x[3])
+    # ... and by norm: a row of dV is a sum of products whose operands are rounded once, so it is off by well under a step of the type, as far as fp16 can
+    # show the result at all
+    for name in ("dk", "dv"):
+        w = want[name][0][:, L // 2:].transpose(1, 2)
+        e = (got[name].double()[:, L // 2:].transpose(1, 2) - w).norm(dim=-1)
+        assert bool((e <= 4 * half_step(torch.float16) * w.norm(dim=-1) + math.sqrt(D) * 2.0 ** -25).all()), (name, float((e / w.norm(dim=-1)).max()))
+
+
+def test_fp16_gradients_of_a_long_uniform_attention():
+    """Probabilities of 1 / 40000, under fp16's smallest normal number."""
+    H, D, Lq, Lk = 1, 32, 40, 40000
+    g = _gen(33)
+    q = torch.randn(1, Lq, H, D, generator=g, device="cuda") * 0.01
+    k, v = (torch.randn(1, Lk, H, D, generator=g, device="cuda") for _ in range(2))
+    dout = torch.randn(1, Lq, H, D, generator=g, device="cuda") * 2.0 ** 12
+    _hold(*(x.half() for x in (q, k, v)), torch.zeros(32, H, device="cuda"), dout.half())
