@@ -65,12 +65,14 @@ class GraphedForward:
         return device.type == "cuda" and os.environ.get("MFAR_ENCODE_GRAPHS", "0") == "1"
 
     def signature(self):
-        """Where the parameters live.  A graph holds addresses: after `.to()`, `load_state_dict(assign=True)` or a dtype change the old ones
-        are stale (in-place updates are fine)."""
-        return tuple((p.data_ptr(), p.dtype) for p in self.encoder.parameters())
+        """Where the parameters live, and which forward runs on them.  A graph holds addresses: after `.to()`, `load_state_dict(assign=True)` or a
+        dtype change the old ones are stale (in-place updates are fine); and it holds the kernels of the attention that was switched on
+        (`use_fused_attention`) when it was captured."""
+        fused = any(getattr(m, "fused_stack", ()) for m in self.encoder.modules())
+        return (fused,) + tuple((p.data_ptr(), p.dtype) for p in self.encoder.parameters())
 
     def begin(self) -> None:
-        """Start of an encode: drop graphs whose parameters moved."""
+        """Start of an encode: drop graphs whose parameters moved or whose attention was switched."""
         sig = self.signature()
         if sig != self.sig:
             self.reset()
