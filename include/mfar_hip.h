@@ -506,7 +506,8 @@ int mfar_pipeline_lists(mfar_pipeline* p, int64_t ticket, int64_t* field_ids, fl
  * Attention with a learned relative position bias by buckets (the gtr-t5 encoder's attention, modeling/util.py:22-36):
  *   S[q][k] = scale <q, k> + table[bucket(k - pos(q))][h] over the visible keys, out = softmax(S) v;  pos(q) = q_start + q.
  * A key is visible if key_mask (1 byte per key, 0 = hidden) leaves it and, when causal, k <= pos(q).  A row without visible keys gives zeros
- * (and zero gradients); hidden keys may hold anything.
+ * (and zero gradients).  A key that no query sees may hold anything and gets zero gradients; one that some query sees holds finite numbers (its
+ * probability of 0 for the others multiplies them).
  * Buckets: `each` = half of a side's buckets hold one distance each, distance d >= each falls into each + (number of borders <= d).  Causal: one
  * side (distances behind the query); otherwise the upper half of the buckets is for keys behind the query's position.
  */

@@ -824,7 +824,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_att
     const int start = at_start(p, b);
     const int key0 = place.tile * AT_COLS, key = key0 + wave * 32 + (l & 31);
     const bool live = key < p.Lk;
-    const bool seen = live && (!p.mask || p.mask[(long long)b * p.mask_b + key] != 0);
+    const bool seen = live && (!p.causal || key < start + p.Lq) && (!p.mask || p.mask[(long long)b * p.mask_b + key] != 0);
     const int col_lo = key0 + wave * 32;
     f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
     const float c = p.scale * LOG2E;

@@ -150,7 +150,8 @@ def relative_bias_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, t
 
     q [B, Lq, H, D], k and v [B, Lk, H, D], float32 / float16 / bfloat16 on one GPU, D <= 128 (any strides; copied where the last dim is not
     contiguous or rows do not start on 16 bytes).  table [num_buckets, H]: the weight of the bias embedding, of any float type (used in fp32).
-    key_mask [B, Lk] bool or uint8: False hides a key from every query; hidden keys may hold anything.  A query that sees no key gets zeros.
+    key_mask [B, Lk] bool or uint8: False hides a key from every query.  A query that sees no key gets zeros.  Keys that no query sees may hold
+    anything; those that some query sees hold finite numbers.
     causal: keys behind a query's position are hidden and all buckets serve the distances back.  q_start: position of the first query among the
     keys, one number or one int32 / int64 [B] tensor -- a decoder's next token over a cache of n keys sits at n - 1.
     max_distance: distances from there on share the last bucket (at most 1023 may be told apart).  scale: 1 as the T5 family has it.

@@ -134,3 +134,22 @@ def test_fp16_gradients_of_a_long_uniform_attention():
     k, v = (torch.randn(1, Lk, H, D, generator=g, device="cuda") for _ in range(2))
     dout = torch.randn(1, Lq, H, D, generator=g, device="cuda") * 2.0 ** 12
     _hold(*(x.half() for x in (q, k, v)), torch.zeros(32, H, device="cuda"), dout.half())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("Lq,Lk,start", [(40, 100, 0), (130, 300, 20), (70, 129, 58), (3, 200, 60)])
+def test_keys_past_every_query_may_hold_anything(dtype, Lq, Lk, start):
+    """Causal: what lies behind the last query's position reaches nothing, and gets zero gradients."""
+    B, H, D = 2, 2, 64
+    g = _gen(34)
+    q = (torch.randn(B, Lq, H, D, generator=g, device="cuda") * 0.2).to(TYPES[dtype])
+    k, v = (torch.randn(B, Lk, H, D, generator=g, device="cuda").to(TYPES[dtype]) for _ in range(2))
+    dout = torch.randn(B, Lq, H, D, generator=g, device="cuda").to(TYPES[dtype])
+    table = torch.randn(32, H, generator=g, device="cuda")
+    end = start + Lq
+    k[:, end:], v[:, end:] = 0.0, 0.0
+    want = _run(q, k, v, table, dout, causal=True, q_start=start)
+    k[:, end:], v[:, end:] = float("nan"), float("inf")
+    got = _run(q, k, v, table, dout, causal=True, q_start=start)
+    assert all(torch.equal(got[n], want[n]) for n in got)
+    assert not got["dk"][:, end:].any() and not got["dv"][:, end:].any() and bool(got["dk"].isfinite().all())
