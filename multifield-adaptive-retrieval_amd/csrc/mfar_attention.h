@@ -338,7 +338,9 @@ __device__ __forceinline__ void at_bias(f32x16& s, const float* lut, int sat, fl
 struct AtSoftmax {
     float base = 0.0f, limit = -__builtin_inff(), sum = 0.0f;               // sum: this half's part
 };
-// N tiles of 32 x 32 scores into the softmax and O' += V' P' with the rows of vt.
+// N tiles of 32 x 32 scores into the softmax and O' += V' P' with the rows of vt.  The sum is of the probabilities as they are multiplied: what rounding
+// added to one that stands far ahead of the rest cancels in the quotient (summed unrounded, such a query's output was off by a half step more than its
+// own rounding).  KEEP multiplies them in two parts, exact to u^2, and sums them unrounded.
 template <typename T, int DP, bool KEEP, int N>
 __device__ __forceinline__ void at_softmax(f32x16 (&s)[N], T* vt, AtSoftmax& m, f32x16* acc) {
     float top = -__builtin_inff();
@@ -365,8 +367,11 @@ __device__ __forceinline__ void at_softmax(f32x16 (&s)[N], T* vt, AtSoftmax& m, 
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             s[t][i] = exp2_fast(s[t][i]);
-            part[i & 1] += s[t][i];
+            if (KEEP || sizeof(T) == 4) part[i & 1] += s[t][i];
         }
+        if constexpr (!KEEP && sizeof(T) == 2)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) part[g] = add_up(at_pack<T>(s[t], g), 0.0f);
         m.sum += part[0] + part[1];
         if (sizeof(T) == 2) __builtin_amdgcn_s_setprio(1);                 // (matrix work first: the other waves' exponentials fill the gaps; 3 % at 8 x 4096)
 #pragma unroll

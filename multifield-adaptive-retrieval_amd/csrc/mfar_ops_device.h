@@ -37,6 +37,23 @@ __device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
     return c;
 }
 
+// c + the 8 elements, two at a time in the dot unit (fp16's smallest numbers count; each pair is added with an error under a step of fp32, so
+// sums that run long take the result in by an ordinary addition)
+__device__ __forceinline__ float add_up(f16x8 x, float c) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) c = __builtin_amdgcn_fdot2(f16x2{x[j], x[j + 1]}, one, c, false);
+    return c;
+}
+__device__ __forceinline__ float add_up(bf16x8 x, float c) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) c = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[j], x[j + 1]}, one, c, false);
+    return c;
+}
+
 // the two halves' values of a column, in either half (v_permlane32_swap: no LDS round trip)
 __device__ __forceinline__ void both_halves(float x, float& a, float& b) {
     typedef u32 u32x2 __attribute__((ext_vector_type(2)));

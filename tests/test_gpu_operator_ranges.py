@@ -153,3 +153,29 @@ def test_keys_past_every_query_may_hold_anything(dtype, Lq, Lk, start):
     got = _run(q, k, v, table, dout, causal=True, q_start=start)
     assert all(torch.equal(got[n], want[n]) for n in got)
     assert not got["dk"][:, end:].any() and not got["dv"][:, end:].any() and bool(got["dk"].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,Lq", [(4, 9), (140, 130)])
+def test_outputs_of_a_query_with_one_key_ahead_of_the_rest(dtype, B, Lq):
+    """Two visible keys a tile apart, the second 2^4 to 2^7.9 times as likely as the first, which set the softmax's base.  Probabilities are multiplied as the type
+    holds them (p1', p2') and divided by the sum of just those, so with w = p2' / (p1' + p2') the roundings of both all but cancel: w is off by at
+    most 2 u w (1 - w), and the output beside that by its own rounding."""
+    H, D, Lk = 2, 64, 160
+    u = half_step(TYPES[dtype])
+    g = _gen(35)
+    mask = torch.zeros(B, Lk, dtype=torch.bool, device="cuda")
+    mask[:, 3], mask[:, 140] = True, True
+    q, k = torch.zeros(B, Lq, H, D, device="cuda"), torch.zeros(B, Lk, H, D, device="cuda")
+    q[..., 0] = (torch.rand(B, Lq, H, generator=g, device="cuda") * 3.9 + 4) * math.log(2)
+    k[:, 140, :, 0] = 1.0
+    v = torch.randn(B, Lk, H, D, generator=g, device="cuda")
+    q, k, v = (x.to(TYPES[dtype]) for x in (q, k, v))
+    from mfar.modeling.attention import relative_bias_attention
+    with torch.no_grad():
+        got = relative_bias_attention(q, k, v, torch.zeros(32, H, device="cuda"), key_mask=mask).double()
+    w = torch.sigmoid(q[..., :1].double())                               # of the second key
+    a, b = v[:, 3].double()[:, None], v[:, 140].double()[:, None]
+    want = a + w * (b - a)
+    f = 64 * U32 * 7
+    check("out", got, want, u * want.abs() * (1 + 4 * u) + (2 * u * (1 + 4 * u) * w * (1 - w) + f) * (a.abs() + b.abs()) + (2.0 ** -25 if dtype == "fp16" else 0.0))
