@@ -51,7 +51,8 @@ def build(flags: dict, freeze_encoder: bool = False) -> SimpleNamespace:
     model_id = f.get("model_path") or f["model_name"]
     tokenizer, encoder, _ = prepare_model(model_id, normalize=f["normalize"], with_decoder=False, freeze_encoder=freeze_encoder)
     encoder.to(device)
-    # MFAR_FUSED_ATTENTION=1: the gtr-t5 encoders run the fused relative-bias attention (training and encoding); other encoders refuse it
+    # MFAR_FUSED_ATTENTION=1: the gtr-t5 encoders run the fused relative-bias attention; other encoders refuse it.  Encoding always; training only
+    # where the model's config has dropout_rate 0 (gtr-t5's has 0.1: its training forwards stay stock, with a warning)
     if os.environ.get("MFAR_FUSED_ATTENTION", "0") == "1":
         encoder.use_fused_attention()
     corpus, vectors_dict, indices_dict = read_and_create_indices(f"{f['corpus']}/corpus", f["dataset_name"], field_info,

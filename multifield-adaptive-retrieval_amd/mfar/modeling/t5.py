@@ -28,6 +28,13 @@ def attention_dropout(stack: torch.nn.Module) -> float:
     return max(float(b.layer[0].SelfAttention.dropout) for b in stack.block)
 
 
+def stays_stock(stack: torch.nn.Module) -> str:
+    """Why a forward of this stack, as it stands, is the stock model's to run; empty: the fused one runs it."""
+    if stack.training and attention_dropout(stack) > 0:
+        return "the encoder is in training mode and drops attention weights, which the kernel does not"
+    return ""
+
+
 def _held(h: torch.Tensor) -> torch.Tensor:
     """Hidden states of an fp16 model stay within the type, as the stock blocks keep them: a sum past the largest value would be infinite, and NaN
     from the next norm on."""

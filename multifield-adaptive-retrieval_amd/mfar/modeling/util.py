@@ -11,6 +11,7 @@ structural only.
 np.memmap file + CPU DenseFlatIndex per field (modeling/util.py:84-101).
 """
 import os
+import warnings
 from pathlib import Path
 from typing import Dict, List, Optional, Tuple
 
@@ -31,14 +32,18 @@ class _Transformer(torch.nn.Module):
     def __init__(self, auto_model):
         super().__init__()
         self.auto_model = auto_model
+        self.told = set()            # reasons for the stock attention that were warned of
         self.fused_stack = ()        # (the T5 stack whose forward mfar/modeling/t5.py runs,); in a tuple: no second registration of its parameters
 
     def forward(self, features):
         if self.fused_stack and features["input_ids"].is_cuda:
-            from mfar.modeling.t5 import attention_dropout, t5_encoder_forward
-            stack = self.fused_stack[0]
-            if not (stack.training and attention_dropout(stack) > 0):
-                return t5_encoder_forward(stack, features["input_ids"], features["attention_mask"])
+            from mfar.modeling.t5 import stays_stock, t5_encoder_forward
+            why = stays_stock(self.fused_stack[0])
+            if not why:
+                return t5_encoder_forward(self.fused_stack[0], features["input_ids"], features["attention_mask"])
+            if why not in self.told:
+                self.told.add(why)
+                warnings.warn(f"the fused attention is switched on, but {why}: these forwards run the stock attention")
         out = self.auto_model(input_ids=features["input_ids"], attention_mask=features["attention_mask"],
                               **({"token_type_ids": features["token_type_ids"]} if "token_type_ids" in features else {}))
         return out[0] if not hasattr(out, "last_hidden_state") else out.last_hidden_state
@@ -77,8 +82,9 @@ class SentenceEncoder(torch.nn.Sequential):
 
     def use_fused_attention(self, enabled: bool = True) -> None:
         """T5 encoders only (ValueError otherwise): forwards on the GPU go through the fused attention, forward and backward
-        (mfar/modeling/t5.py).  A training forward that drops attention weights (`dropout_rate` > 0 in train mode) stays with the stock attention:
-        the kernel has no dropout."""
+        (mfar/modeling/t5.py).  A training forward that drops attention weights (`dropout_rate` > 0 in train mode, which gtr-t5 has) stays with the
+        stock attention, with a warning once: the kernel has no dropout.  To train through the fused attention, set `dropout` of the attention
+        modules (`encoder.auto_model.encoder.block[i].layer[0].SelfAttention`) to 0, or `dropout_rate` in the model's config."""
         from mfar.modeling.t5 import t5_stack
         self[0].fused_stack = (t5_stack(self.auto_model),) if enabled else ()
 

@@ -19,3 +19,14 @@ def test_captured_forwards_are_dropped_when_the_attention_is_switched():
             graphed.sig = graphed.signature()
         graphed.begin()
         assert bool(graphed.graphs) == (on == before), on
+
+
+def test_why_a_forward_stays_stock():
+    from mfar.modeling.t5 import attention_dropout, stays_stock, t5_stack
+    stack = t5_stack(_t5().auto_model)
+    assert attention_dropout(stack) > 0 and not stack.training and not stays_stock(stack)
+    stack.train()
+    assert "drops attention weights" in stays_stock(stack)
+    for block in stack.block:
+        block.layer[0].SelfAttention.dropout = 0.0
+    assert not stays_stock(stack)                                          # (the dropout of hidden states is the stock modules' own)
