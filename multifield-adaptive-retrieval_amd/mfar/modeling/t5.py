@@ -28,11 +28,28 @@ def attention_dropout(stack: torch.nn.Module) -> float:
     return max(float(b.layer[0].SelfAttention.dropout) for b in stack.block)
 
 
-def stays_stock(stack: torch.nn.Module) -> str:
-    """Why a forward of this stack, as it stands, is the stock model's to run; empty: the fused one runs it."""
+def stays_stock(auto_model: torch.nn.Module, stack: torch.nn.Module) -> str:
+    """Why a forward of this model, as it stands, is the stock model's to run; empty: the fused one runs it."""
+    if getattr(auto_model, "encoder", auto_model) is not stack:
+        return "the encoder's model is another than the one it was switched on for"
     if stack.training and attention_dropout(stack) > 0:
         return "the encoder is in training mode and drops attention weights, which the kernel does not"
+    if stack.training and any(getattr(m, "gradient_checkpointing", False) for m in (stack, *stack.block)):
+        return "gradient checkpointing is on, which goes through the stock blocks"
+    for m in (auto_model, *_passed_by(stack)):
+        if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or "forward" in vars(m):
+            return f"a {type(m).__name__} that it passes by has hooks or a forward of its own"
     return ""
+
+
+def _passed_by(stack: torch.nn.Module):
+    """The modules whose own forward the fused one does not call."""
+    yield stack
+    for block in stack.block:
+        yield block
+        yield block.layer[0]
+        yield block.layer[0].SelfAttention
+    yield stack.block[0].layer[0].SelfAttention.relative_attention_bias
 
 
 def _held(h: torch.Tensor) -> torch.Tensor:

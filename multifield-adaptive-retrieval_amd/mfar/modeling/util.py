@@ -38,7 +38,7 @@ class _Transformer(torch.nn.Module):
     def forward(self, features):
         if self.fused_stack and features["input_ids"].is_cuda:
             from mfar.modeling.t5 import stays_stock, t5_encoder_forward
-            why = stays_stock(self.fused_stack[0])
+            why = stays_stock(self.auto_model, self.fused_stack[0])
             if not why:
                 return t5_encoder_forward(self.fused_stack[0], features["input_ids"], features["attention_mask"])
             if why not in self.told:

@@ -52,3 +52,24 @@ def test_train_command_with_the_fused_attention(tmp_path, monkeypatch, dropout):
         assert True in runs and not told, (runs, told)
         table = m.encoder.auto_model.encoder.block[0].layer[0].SelfAttention.relative_attention_bias.weight
         assert table.requires_grad and bool(table.isfinite().all())
+
+
+def test_hooks_on_attention_modules_run():
+    """A forward hook on an attention module sees its outputs, the fused attention switched on or not."""
+    import torch
+    from mfar.modeling.util import prepare_model
+    _, enc, _ = prepare_model("random-init-t5:64x2")
+    enc = enc.cuda()
+    f = {k: v.cuda() for k, v in enc.tokenize(["alpha beta", "gamma"]).items() if k in ("input_ids", "attention_mask")}
+    with torch.no_grad():
+        want = enc(f)["sentence_embedding"]
+    enc.use_fused_attention()
+    seen = []
+    handle = enc.auto_model.encoder.block[1].layer[0].SelfAttention.register_forward_hook(lambda m, i, o: seen.append(1))
+    with torch.no_grad(), pytest.warns(UserWarning, match="T5Attention"):
+        assert torch.equal(enc(f)["sentence_embedding"], want)
+    assert seen == [1]
+    handle.remove()
+    with torch.no_grad():
+        enc(f)
+    assert seen == [1]
