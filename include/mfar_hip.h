@@ -543,7 +543,8 @@ int mfar_attention_backward(int device, const mfar_attention* a, void* stream); 
  * 8-bit products with a scale for each token (row of x) and each output channel.
  *   mfar_quantize_rows: scale[m] = max|x[m]| times 1 / 127 (both rounded to fp32), q[m] = rint(x[m] / scale[m]), ties to even; rows of q ldq bytes apart.  A row of zeros gets
  *   scale 0, a row with an infinity or NaN scale NaN and zeros.
- *   mfar_int8_linear: y = quantize_rows(x) wq' scaled by both scales (+ bias), rounded once to y's type.
+ *   mfar_int8_linear: y = quantize_rows(x) wq' scaled by both scales (+ bias).  The integer sums are exact; a sum's conversion to fp32, its products
+ *   with the row's and the channel's scale and the sum with the bias each round to fp32, the result to y's type.
  * x [M, K] rows ldx elements apart; wq [N, K] contiguous, 16-byte aligned; w_scale [N]; bias [N] fp32 or NULL; y [M, N] contiguous, of any of the three types.
  * K <= 131072; M, N <= 2^23.
  */

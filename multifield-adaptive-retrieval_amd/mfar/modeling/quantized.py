@@ -44,7 +44,8 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [..., K] times 8-bit weights wq [N, K] with one scale per channel w_scale [N] (+ bias [N]) -> [..., N] of out_dtype (x's type if not
-    given), every token quantised by its own scale on the way (`quantize_rows`); rounded once."""
+    given), every token quantised by its own scale on the way (`quantize_rows`).  The integer sums are exact; their conversion to fp32, the products
+    with both scales and the sum with the bias each round to fp32, the result to its type."""
     dev = _native.op_device(x, wq, w_scale, bias)
     _check(x)
     K = x.shape[-1]
