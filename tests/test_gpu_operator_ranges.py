@@ -179,3 +179,29 @@ def test_outputs_of_a_query_with_one_key_ahead_of_the_rest(dtype, B, Lq):
     want = a + w * (b - a)
     f = 64 * U32 * 7
     check("out", got, want, u * want.abs() * (1 + 4 * u) + (2 * u * (1 + 4 * u) * w * (1 - w) + f) * (a.abs() + b.abs()) + (2.0 ** -25 if dtype == "fp16" else 0.0))
+
+
+@pytest.mark.parametrize("dtype,D", [("fp32", 64), ("fp32", 128), ("fp16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_large_batches_over_more_than_4096_keys(dtype, D, causal):
+    """The kernels of large batches across a group of 4096 keys, forward and backward, in fp32 and wide heads too, where LDS holds one step of tiles alone: keys
+    hidden on either side of the border, up to it, behind it, and all of a group."""
+    from helpers.operator_refs import attention_ref
+    B, H, Lq, Lk = 64, 2, 35, 4230
+    print(f"attention {dtype} {D} {causal}", flush=True)
+    g = _gen(36)
+    q = (torch.randn(B, Lq, H, D, generator=g, device="cuda") * (1.5 / math.sqrt(D))).to(TYPES[dtype])
+    k, v = (torch.randn(B, Lk, H, D, generator=g, device="cuda").to(TYPES[dtype]) for _ in range(2))
+    dout = torch.randn(B, Lq, H, D, generator=g, device="cuda").to(TYPES[dtype])
+    table = torch.randn(32, H, generator=g, device="cuda")
+    mask = torch.rand(B, Lk, generator=g, device="cuda") < 0.7
+    mask[0] = True
+    mask[1, 4096:], mask[2, :4096], mask[3, 4095:4097] = False, False, False
+    mask[4], mask[5, :] = False, False
+    mask[5, 4096] = True
+    mask[6, 4090:], mask[6, 4100] = False, True
+    start = Lk - Lq - 3 if causal else 0
+    got = _run(q, k, v, table, dout, key_mask=mask, causal=causal, q_start=start)
+    for name, (want, bound) in attention_ref(q, k, v, table, mask, causal, 128, start, 1.0, dout).items():
+        check(name, got[name], want, bound)
+    assert not got["out"][4].any() and not got["dk"][4].any()
