@@ -340,8 +340,8 @@ struct AtSoftmax {
 };
 // N tiles of 32 x 32 scores into the softmax and O' += V' P' with the rows of vt.  The sum is of the probabilities as they are multiplied: what rounding
 // added to one that stands far ahead of the rest cancels in the quotient (summed unrounded, such a query's output was off by a half step more than its
-// own rounding).  KEEP multiplies them in two parts, exact to u^2, and sums them unrounded.
-template <typename T, int DP, bool KEEP, int N>
+// own rounding).  TWO multiplies them in two parts, exact to u^2, and sums them unrounded.
+template <typename T, int DP, bool TWO, int N>
 __device__ __forceinline__ void at_softmax(f32x16 (&s)[N], T* vt, AtSoftmax& m, f32x16* acc) {
     float top = -__builtin_inff();
 #pragma unroll
@@ -367,9 +367,9 @@ __device__ __forceinline__ void at_softmax(f32x16 (&s)[N], T* vt, AtSoftmax& m, 
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             s[t][i] = exp2_fast(s[t][i]);
-            if (KEEP || sizeof(T) == 4) part[i & 1] += s[t][i];
+            if (TWO || sizeof(T) == 4) part[i & 1] += s[t][i];
         }
-        if constexpr (!KEEP && sizeof(T) == 2)
+        if constexpr (!TWO && sizeof(T) == 2)
 #pragma unroll
             for (int g = 0; g < 2; ++g) part[g] = add_up(at_pack<T>(s[t], g), 0.0f);
         m.sum += part[0] + part[1];
@@ -380,7 +380,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&s)[N], T* vt, AtSoftmax& m, 
             for (int g = 0; g < 2; ++g) {
                 const V8<T> vf = at_cols<T, DP>(vt, 32 * t, g, dt);
                 acc[dt] = mma(vf, at_pack<T>(s[t], g), acc[dt]);
-                if (KEEP) acc[dt] = mma(vf, at_pack_lo<T>(s[t], g), acc[dt]);
+                if (TWO) acc[dt] = mma(vf, at_pack_lo<T>(s[t], g), acc[dt]);
             }
         if (sizeof(T) == 2) __builtin_amdgcn_s_setprio(0);
     }
@@ -399,8 +399,8 @@ __device__ __forceinline__ float at_norm(float sum) { return sum > 0.0f ? 1.0f /
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // Bound by the vector unit: an exponential, the bias, a maximum, a sum and half a conversion a score, beside 8 matrix instructions a tile of 32 x 32
 // (64 x 512 x 12 heads x 64 fp16, padded: 73 us; 8 x 4096: 510 us, 800 TFLOP/s; keeping what the backward pass needs: 53 us for 32 x 512, 700 for 8 x 4096).
-// KEEP (training, 16-bit types): D = <dO, O> of the backward pass enters the bias table's fp32 gradient, a difference of large sums.  P V takes
-// P in two parts (value and what its rounding dropped, error u^2) and out_lo keeps what the output's rounding dropped.
+// KEEP (training, 16-bit types): D = <dO, O> of the backward pass enters every score gradient as the part that P dP is reduced by, and so dQ, dK and, in
+// fp32, the bias table's gradient, all differences of large sums.  P V takes P in two parts (value and what its rounding dropped, error u^2) and out_lo keeps what the output's rounding dropped.
 template <typename T, int DP, bool KEEP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_attn_forward_kernel(const AttnParams p) {
     AtPlace place;
@@ -465,7 +465,8 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
 // ---- forward, few queries (short texts, a decoder's next token, small batches): the work of 32 queries is divided over the keys --------------------
 // Tiles of 32 keys go to the waves in turn, 4 waves a block and `splits` blocks per (batch, head): K and V in whole rows through LDS of the
 // wave's own, no barrier in the loop, the next tile's loads in flight.  The waves' partial softmaxes are joined in LDS, the blocks' in a second
-// launch, both in a fixed order.  Bound by reading K and V (16 ragged caches of 4097 x 12 heads x 64 bf16, 113 MB: 28 us, and 4 to join) and, for a short
+// launch, both in a fixed order.  The matrix unit has time for P in two parts (serving alone: 16 caches of 4097 25.1 -> 25.7 us, a short text 6.2 -> 6.3), so
+// outputs are as exact as from an fp32 P.  Bound by reading K and V (16 ragged caches of 4097 x 12 heads x 64 bf16, 113 MB: 28 us, and 4 to join) and, for a short
 // text, by latency (12 x 12 heads x 64: 6 us).
 struct AttnSplit {
     float *o, *ml;               // [rows, splits, D], [rows, splits, 2] (maximum, sum); row = (batch * Lq + query) * H + head
@@ -542,7 +543,7 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
         if (seen) {
             at_bias<1>(s[0], lut, p.sat, c, row0, col, start + q0, p.causal != 0, run.base);
             if (seen != ~0u) at_hide(s[0], seen);
-            at_softmax<T, DP, KEEP, 1>(s, vt, run, acc);
+            at_softmax<T, DP, sizeof(T) == 2, 1>(s, vt, run, acc);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();

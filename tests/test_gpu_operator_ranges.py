@@ -205,3 +205,25 @@ def test_large_batches_over_more_than_4096_keys(dtype, D, causal):
     for name, (want, bound) in attention_ref(q, k, v, table, mask, causal, 128, start, 1.0, dout).items():
         check(name, got[name], want, bound)
     assert not got["out"][4].any() and not got["dk"][4].any()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,Lq,Lk,causal", [(1, 12, 12, False), (5, 1, 4097, True), (3, 31, 300, False), (2, 200, 200, False)])
+def test_outputs_of_few_queries_are_rounded_once(dtype, B, Lq, Lk, causal):
+    """Short texts, single tokens over a cache and small batches: P is multiplied in two parts of the type (u^2 each), so an output is off by its own rounding and
+    what fp32 leaves, element by element, however much of P|V| cancels in it."""
+    from helpers.operator_refs import attention_ref
+    from mfar.modeling.attention import relative_bias_attention
+    H, D = 3, 64
+    g = _gen(37)
+    q = (torch.randn(B, Lq, H, D, generator=g, device="cuda") * (1.5 / math.sqrt(D))).to(TYPES[dtype])
+    k, v = (torch.randn(B, Lk, H, D, generator=g, device="cuda").to(TYPES[dtype]) for _ in range(2))
+    table = torch.randn(32, H, generator=g, device="cuda")
+    start = Lk - Lq if causal else 0
+    with torch.no_grad():
+        got = relative_bias_attention(q, k, v, table, causal=causal, q_start=start)
+    u = half_step(TYPES[dtype])
+    want, loose = attention_ref(q, k, v, table, None, causal, 128, start, 1.0)["out"]
+    # P|V| from above: `loose` holds it at least u times; scores are under 9, fp16's two parts miss 2^-31 of the largest P at most
+    f = (4 * u * u + 64 * 10 * U32) * loose / u
+    check("out", got, want, u * want.abs() + f + (2.0 ** -24 if dtype == "fp16" else 0.0))
