@@ -517,7 +517,7 @@ typedef struct mfar_attention {
     int32_t causal, n_buckets, n_borders;   /* n_buckets <= 256 (even unless causal) */
     float scale;
     const int32_t* borders;                 /* HOST [n_borders], ascending: n_borders = side - side / 2 - 1; last (or each) <= 1023 */
-    const float* table;                     /* [n_buckets, H] fp32 */
+    const float* table;                     /* [n_buckets, H] fp32: numbers of up to 1e38, or -infinity */
     const void *q, *k, *v;                  /* element (b, l, h, d) at b * x_b + l * x_l + h * x_h + d; base and strides multiples of 16 bytes; x_l in 0..2^22 */
     int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;
     const uint8_t* key_mask;                /* [B, Lk] rows mask_b apart, or NULL: all visible */

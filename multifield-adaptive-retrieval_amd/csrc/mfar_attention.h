@@ -12,8 +12,9 @@
 // keys in lanes for dK / dV; each recomputes P from the stored log2-sum of the forward pass.  No float atomics on shared addresses: results
 // do not change from run to run.
 // P and dS are rounded to the inputs' type on their way into a product (the matrix unit takes nothing wider at its rate): half a step each, in fp16
-// whatever their size (AtFit), independent from key to key, which adds to dQ and dK about what the rounding of those results does (2.9e-4 from the 64-bit gradient for 2.1e-4 in fp16; bf16
-// over two keys 2.9e-3 for 1.7e-3).  Sums stay in fp32, the table's gradient takes dS unrounded.
+// whatever their size (AtFit), independent from key to key, which adds to dQ and dK about what the rounding of those results does (2.9e-4 from the
+// 64-bit gradient for 2.1e-4 in fp16; bf16 over two keys 2.9e-3 for 1.7e-3) and to the outputs of large batches a quarter of it (2.6e-4 for 2.1e-4).
+// Where there is time, and where a backward pass follows, P goes in two parts.  Sums stay in fp32, the table's gradient takes dS unrounded.
 //
 // The bias of a (query, key) pair depends on k - pos(q) alone and is constant beyond `sat` (the first distance of the last bucket): a table
 // of 2 sat + 1 values per head lives in LDS, and a tile whose distances all lie beyond sat adds one constant.
@@ -397,8 +398,10 @@ __device__ __forceinline__ float at_rounded(float x) {
 __device__ __forceinline__ float at_norm(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }   // no keys: zeros; NaN stays
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
-// Bound by the vector unit: an exponential, the bias, a maximum, a sum and half a conversion a score, beside 8 matrix instructions a tile of 32 x 32
-// (64 x 512 x 12 heads x 64 fp16, padded: 73 us; 8 x 4096: 510 us, 800 TFLOP/s; keeping what the backward pass needs: 53 us for 32 x 512, 700 for 8 x 4096).
+// At long lengths bound by the vector unit: an exponential, the bias, a maximum, a sum and half a conversion a score, beside 8 matrix instructions a tile of
+// 32 x 32 (8 x 4096 x 12 heads x 64 fp16: 530 us, 780 TFLOP/s; keeping what the backward pass needs, 4 x 4096: 366 us).  At 512 keys a block lives for up to 8
+// tiles, and about half of its time is what lies before and behind them: the first loads, mask, bias table, results (64 x 512, padded: 74 us, 400
+// TFLOP/s; 32 x 512 keeping: 53 us ragged, 60 full).
 // KEEP (training, 16-bit types): D = <dO, O> of the backward pass enters every score gradient as the part that P dP is reduced by, and so dQ, dK and, in
 // fp32, the bias table's gradient, all differences of large sums.  P V takes P in two parts (value and what its rounding dropped, error u^2) and out_lo keeps what the output's rounding dropped.
 template <typename T, int DP, bool KEEP>
@@ -466,8 +469,8 @@ __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_att
 // Tiles of 32 keys go to the waves in turn, 4 waves a block and `splits` blocks per (batch, head): K and V in whole rows through LDS of the
 // wave's own, no barrier in the loop, the next tile's loads in flight.  The waves' partial softmaxes are joined in LDS, the blocks' in a second
 // launch, both in a fixed order.  The matrix unit has time for P in two parts (serving alone: 16 caches of 4097 25.1 -> 25.7 us, a short text 6.2 -> 6.3), so
-// outputs are as exact as from an fp32 P.  Bound by reading K and V (16 ragged caches of 4097 x 12 heads x 64 bf16, 113 MB: 28 us, and 4 to join) and, for a short
-// text, by latency (12 x 12 heads x 64: 6 us).
+// outputs are as exact as from an fp32 P.  Bound by reading K and V (16 ragged caches of 4097 x 12 heads x 64 bf16, 113 MB:
+// 29 us, and 4 to join) and, for a short text, by latency (12 x 12 heads x 64: 6 us).
 struct AttnSplit {
     float *o, *ml;               // [rows, splits, D], [rows, splits, 2] (maximum, sum); row = (batch * Lq + query) * H + head
     int splits;
@@ -678,7 +681,8 @@ __device__ __forceinline__ float at_refit(float top, AtFit& m) {
 
 // ---- backward: dQ, the bias gradient, D ---------------------------------------------------------------------------------------------------
 // Bound by the vector unit (exponentials, bias, diagonal sums) with the matrix unit behind it at long lengths, by the first loads of a block at short ones:
-// three blocks a CU (32 x 512 x 12 heads x 64 fp16: 84 us, two blocks 94; of it the bias gradient 16; 4 x 4096: 372 us, 830 TFLOP/s).
+// three blocks a CU (32 x 512 x 12 heads x 64 fp16, no mask: 87 us; before dS had a factor for each query 84, and with two blocks a CU 94; of it the bias
+// gradient 16; ragged from 1 / 8 of the length 75; 4 x 4096: 405 us, 760 TFLOP/s).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 3)) void mfar_attn_dq_kernel(const AttnParams p) {
     AtPlace place;
@@ -815,8 +819,9 @@ __global__ __launch_bounds__(AT_BLOCK) void mfar_attn_dtable_kernel(const float*
 }
 
 // ---- backward: dK, dV (keys in lanes) -------------------------------------------------------------------------------------------------------
-// Two blocks a CU: what a third would leave of the registers does not hold two accumulators, K and V (32 x 512 x 12 heads x 64 fp16: 83 us against 95 to
-// 103; 4 x 4096: 465 against 520 to 560).
+// Two blocks a CU: what a third would leave of the registers does not hold two accumulators, K and V (32 x 512 x 12 heads x 64 fp16, no mask, before P and dS had
+// factors: 83 us against 95 to 103; with them 86, ragged from 1 / 8 of the length 81; 4 x 4096: 530 us, 780 TFLOP/s).  Head size 128 spills 53 to 62
+// registers (152 to 212 bytes of scratch).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_BLOCK, at_waves(sizeof(T), DP, 2)) void mfar_attn_dkv_kernel(const AttnParams p) {
     AtPlace place;

@@ -4,8 +4,8 @@
 //   loss = tau^2 sum_k p_k (log p_k - log q[id_k]),      d student[j] = g tau (q_j - sum over k with id_k = j of p_k)
 //
 // Bound by memory: the forward pass reads the student's scores once (running maximum and sum, in the log2 domain), the backward pass reads
-// them again and writes the gradient (64 x 500009 fp32: 31 us, 4.1 TB/s, and 47, 5.4 TB/s; 4096 x 32005 bf16: 95, where the exponentials count, and
-// 97).  A row is split over blocks when there are few rows; partial (maximum, sum) pairs are joined in a
+// them again and writes the gradient (64 x 500009 fp32: 31 us, 4.1 TB/s, and 47, 5.4 TB/s; 4096 x 32005 bf16: 94, 2.8 TB/s, and 98.  There a row is 4
+// turns of a block, and the teacher's fetch and four reductions over the block around them overlap with nothing; the arithmetic itself comes to some 30 us).  A row is split over blocks when there are few rows; partial (maximum, sum) pairs are joined in a
 // second launch, in block order.  A listed column's gradient is written once, from its sum over the list in list order: no atomics.
 // An id >= N makes the row's loss and gradient NaN.
 #pragma once

@@ -149,7 +149,9 @@ def relative_bias_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, t
     """softmax(scale q k' + table[bucket(key position - query position)]) v per head -> [B, Lq, H, D], differentiable in q, k, v and table.
 
     q [B, Lq, H, D], k and v [B, Lk, H, D], float32 / float16 / bfloat16 on one GPU, D <= 128 (any strides; copied where the last dim is not
-    contiguous or rows do not start on 16 bytes).  table [num_buckets, H]: the weight of the bias embedding, of any float type (used in fp32).
+    contiguous or rows do not start on 16 bytes).  table [num_buckets, H]: the weight of the bias embedding, of any float type (used in fp32; numbers of
+    up to 1e38 or -infinity).  Scores and their rows' logarithms are fp32 numbers: a probability in the backward pass is off by up to 2^-18 of the row's
+    largest score, relative, so a table is no place for masks by large negative numbers where a row may hold nothing else.
     key_mask [B, Lk] bool or uint8: False hides a key from every query.  A query that sees no key gets zeros.  Keys that no query sees may hold
     anything; those that some query sees hold finite numbers.
     causal: keys behind a query's position are hidden and all buckets serve the distances back.  q_start: position of the first query among the
